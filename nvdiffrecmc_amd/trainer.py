@@ -852,11 +852,10 @@ class DirectLightingStep:
             # same; this runtime does not capture them: torch refuses external events on ROCm, and hipStreamWaitEvent(.., hipEventWaitExternal)
             # on a capturing stream joins the recording stream into the capture instead -- "capturing stream has unjoined work".)
             if getattr(self, '_build_side', None) is None:
-                # HIGH priority: HIP deals its streams to four hardware queues per priority level, and a normal-priority stream created
-                # late in a process may share the main stream's queue -- the first measurement of this schedule showed the main stream
-                # standing still for the whole rebuild (tools/side_graph_probe.py: one in four fresh normal streams serialises with the
-                # main stream, none of the high-priority ones does); the rebuild is on the traversal's critical path anyway
-                self._build_side = torch.cuda.Stream(device=self.dev, priority=-1)
+                # The DEFAULT priority: work on streams of different priorities has hung on this runtime for good.  HIP deals its streams
+                # to four hardware queues, so one in four late streams shares the main stream's queue and the rebuild then runs in line
+                # with it (tools/side_graph_probe.py) -- slower, the same results.
+                self._build_side = torch.cuda.Stream(device=self.dev)
                 self._ev_build, self._ev_main = torch.cuda.Event(), torch.cuda.Event()
             with _capture_graph(g1):
                 self._build_bvh()

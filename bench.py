@@ -169,6 +169,8 @@ def run(args):
                 dist.init_process_group(backend)
         world = dist.get_world_size()                 # what the collective library actually initialised
     dev = torch.device('cuda', dev_index)
+    from nvdiffrecmc_amd.parallel import collective_device
+    coll_dev = collective_device(dev) if dist is not None else dev     # (a gloo dry run: host tensors)
 
     from nvdiffrecmc_amd.trainer import DirectLightingStep
     from nvdiffrecmc_amd import optixutils as ou
@@ -212,7 +214,7 @@ def run(args):
     def max_over_ranks(x):
         if dist is None:
             return x
-        tt = torch.tensor([x], dtype=torch.float64, device=dev)
+        tt = torch.tensor([x], dtype=torch.float64, device=coll_dev)
         dist.all_reduce(tt, op=dist.ReduceOp.MAX)
         return float(tt.item())
 
@@ -259,7 +261,7 @@ def run(args):
             ext_ms.append(a.elapsed_time(b))
             more = len(ext_ms) < 50 or (time.perf_counter() - t_ext < 3.0 and len(ext_ms) < 2000)
             if dist is not None:     # all ranks must run the same number of collectives: agree on when to stop
-                flag = torch.tensor([1.0 if more else 0.0], device=dev)
+                flag = torch.tensor([1.0 if more else 0.0], device=coll_dev)
                 dist.all_reduce(flag, op=dist.ReduceOp.MAX)
                 more = flag.item() != 0.0
             if not more:
@@ -305,7 +307,7 @@ def run(args):
                                                                      n_samples_x=n, rnd_seed=0)
         bvh2_nodes, bvh2_tris, bvh2_rays = ou.ops.env_shade_traversal_counts.bvh2
         clock_mhz = ou.ops.env_shade_traversal_counts.clock_mhz
-    rays_pass = torch.tensor([step.rays_per_pass(), n_traced], dtype=torch.float64, device=dev)
+    rays_pass = torch.tensor([step.rays_per_pass(), n_traced], dtype=torch.float64, device=coll_dev)
     if dist is not None:
         dist.all_reduce(rays_pass, op=dist.ReduceOp.SUM)
     queries_step_total = 2.0 * float(rays_pass[0].item())  # forward + backward shadow-ray queries (2*S per covered pixel), all ranks

@@ -26,6 +26,11 @@ def shard_views(n_views, rank, world_size):
     return list(range(rank * per, min(n_views, (rank + 1) * per)))
 
 
+def collective_device(device, group=None):
+    """Where a tensor of `device` must lie for a collective of this group: host memory for gloo, the device itself for RCCL."""
+    return torch.device('cpu') if dist.get_backend(group) == 'gloo' else torch.device(device)
+
+
 def allreduce_gradients(params, world_size=None, group=None, average=True, local_weight=None, skip_single=True):
     """Sum (or average: the loss is a mean over the batch of views, renderutils/ops.py:494) the .grad of `params` across ranks
     through ONE flat bucket: a one-chunk GradientExchange, written back into the parameters' own .grad tensors.  Parameters
@@ -218,6 +223,12 @@ class GradientExchange:
 
     # ------------------------------------------------------------------------------------------------------------- collectives
     def _all_reduce(self, t, op):
+        if t.is_cuda and collective_device(t.device, self.group).type == 'cpu':
+            # gloo on device tensors has hung when several ranks share a card: through host memory, with synchronous copies (dry runs only)
+            h = t.cpu()
+            dist.all_reduce(h, op=op, group=self.group)
+            t.copy_(h)
+            return None
         return dist.all_reduce(t, op=op, group=self.group, async_op=True)
 
     def start(self, skip_single=True):

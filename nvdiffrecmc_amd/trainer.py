@@ -938,7 +938,8 @@ class DirectLightingStep:
         launches would still be correct, but the run would no longer be what its bench line says)."""
         if world_size > 1 and _dist_ready():
             import torch.distributed as dist
-            t = torch.tensor([1.0 if ok else 0.0], device=self.dev)
+            from .parallel import collective_device
+            t = torch.tensor([1.0 if ok else 0.0], device=collective_device(self.dev))
             dist.all_reduce(t, op=dist.ReduceOp.MIN)
             return bool(t.item() > 0.5)
         return ok

@@ -104,5 +104,18 @@ __device__ __forceinline__ float fetch1(const View4 &v, int64_t n, int64_t h, in
     return v.p[n * v.s0 + h * v.s1 + w * v.s2];
 }
 
+// buf[0 .. n) = 0 as a kernel: a memset node inside a captured graph has given wrong results on replays after the first, so every launch a
+// caller may capture clears its memory this way.
+static __global__ void __launch_bounds__(256) nvdr_fill_zero_kernel(float *buf, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) buf[i] = 0.0f;
+}
+static inline void nvdr_fill_zero(float *buf, int64_t n, hipStream_t stream)
+{
+    if (n <= 0) return;
+    const int64_t blocks = (n + 1023) / 1024;
+    nvdr_fill_zero_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(buf, n);
+}
+
 static inline int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
 static inline unsigned div_up(int64_t a, int64_t b) { return (unsigned)((a + b - 1) / b); }

@@ -944,7 +944,7 @@ extern "C" int nvdr_gather_rows_fwd(const float *table, const int *index, int64_
 extern "C" int nvdr_gather_rows_bwd(const float *dout, const int *index, int64_t n, int channels, int64_t table_rows, float *dtable, void *stream)
 {
     NVDR_REQUIRE(dout && index && dtable && n >= 0 && channels >= 1 && channels <= 16 && table_rows >= 0, "gather_rows_bwd: bad argument");
-    NVDR_HIP_TRY(hipMemsetAsync(dtable, 0, sizeof(float) * (size_t)table_rows * channels, (hipStream_t)stream));
+    nvdr_fill_zero(dtable, table_rows * channels, (hipStream_t)stream);
     if (n == 0) return 0;
     gather_rows_bwd_kernel<<<div_up(n * channels, 256), 256, 0, (hipStream_t)stream>>>(dout, index, n, channels, dtable);
     NVDR_LAUNCH_CHECK();

@@ -32,7 +32,9 @@ SOURCES = [
 
 # -ffp-contract=off: the sampling math must round exactly like the CPU oracle
 # (see include/nvdr_detmath.h); fused operations are written as explicit fmaf.
-FLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off',
+# -packed-fp32-ops: the compiler makes v_pk_add / mul / fma_f32 from ordinary float code at -O3, and some of their forms have given wrong
+# results now and then on MI355X; the target feature is taken away for every source (the host pass warns that it does not know it).
+FLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-I' + os.path.join(ROOT, 'include'), '-I' + CSRC, '-Wno-unused-result', '-Wno-unused-value'] + os.environ.get('NVDR_EXTRA_FLAGS', '').split()
 
 

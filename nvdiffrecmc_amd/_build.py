@@ -27,6 +27,7 @@ SOURCES = [
     'gbuffer.hip',
     'mesh.hip',
     'optim.hip',
+    'gradnorm.hip',
     'exchange.hip',
 ]
 

@@ -172,6 +172,10 @@ _SIGNATURES = {
     'nvdr_light_update_pdf': [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],
     'nvdr_adam_step': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_void_p],
     'nvdr_adam_step_partial': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p],
+    'nvdr_adam_step_clipped': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p, c_void_p],
+    'nvdr_grad_norm_workspace': [c_int64],
+    'nvdr_grad_norm': [c_void_p, c_void_p, ctypes.c_char_p, c_void_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
+    'nvdr_grad_clip': [c_void_p, c_void_p, ctypes.c_char_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
     'nvdr_abi_sizeof': [c_int],
     'nvdr_tile_flags': [c_void_p, c_int64, c_int, c_void_p, c_void_p],
     'nvdr_tile_plan': [c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
@@ -180,7 +184,7 @@ _SIGNATURES = {
     'nvdr_test_detmath': [c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
     'nvdr_test_arith': [c_void_p, c_void_p],
 }
-_RESTYPES = {'nvdr_last_error': ctypes.c_char_p, 'nvdr_image_loss_num_partials': c_int64, 'nvdr_abi_sizeof': ctypes.c_size_t}
+_RESTYPES = {'nvdr_last_error': ctypes.c_char_p, 'nvdr_image_loss_num_partials': c_int64, 'nvdr_grad_norm_workspace': c_int64, 'nvdr_abi_sizeof': ctypes.c_size_t}
 # nvdr_abi_sizeof(which) -> the ctypes mirror that must have that size (checked once at load: a stale library or a stale mirror is an error)
 _ABI_MIRRORS = {0: 'NvdrAdamTensor', 1: 'NvdrEnvShadeArgs', 2: 'NvdrTextureArgs', 3: 'NvdrInterpolateBwdArgs', 4: 'NvdrTensor', 5: 'NvdrGbufferArgs',
                 6: 'NvdrMeshArgs', 7: 'NvdrBvhInfo'}

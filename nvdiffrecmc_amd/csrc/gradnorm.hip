@@ -1,0 +1,431 @@
+// gradnorm.hip -- the global norm of many gradient tensors, and clipping by it.
+//
+//     norm   = (sum over all tensors k and elements i of |s_k g_ki|^p)^(1/p),  p = 1, 2;  their largest magnitude for p = infinity
+//     factor = min(1, max_norm / (norm + 1e-6))
+//     g      = g * factor          (clip; nothing is written when the factor is one)
+//
+// The gradients of a Monte-Carlo estimate carry outliers (one firefly in one view); clipping bounds the step they can cause.  Bytes bound
+// all of it: the norm reads every gradient once, the scaling reads and writes it.
+//
+// Sums in fp64.  An fp32 gradient's square leaves the range of fp32 from 1.8e19 up and 1e-19 down, and a sum of 1e9 terms loses half of
+// fp32's digits; a conversion and an fma in fp64 per element are far below what the memory can deliver in elements.  No atomics: every
+// workgroup writes its sum to a place of its own and they are added in a fixed order, so that a result depends on the values, the sizes
+// and the alignment alone.
+//
+// Work split.  The tensors are cut into chunks of NVDR_GN_CHUNK bytes; a launch has at most NVDR_GN_GRID workgroups, each of which takes a
+// contiguous run of chunks, whatever tensors they fall into: a long tensor is shared by many workgroups and many short ones by few.  The table
+// of the tensors travels in the kernel arguments -- by value, so that a captured graph keeps it and no copy to the device is needed -- which
+// bounds the tensors of a launch; longer lists take several launches.  Neighbours in memory (views of one bucket) become one entry.
+#include <stdlib.h>
+#include <algorithm>
+
+#include "common.h"
+#include "nvdr_hip.h"
+
+#define NVDR_GN_BLOCK 512
+#define NVDR_GN_GRID 1024
+#define NVDR_GN_TENSORS 160
+#define NVDR_GN_CHUNK 16384
+#define NVDR_GN_EPS 1e-6
+
+enum { GN_INF = 0, GN_ONE = 1, GN_TWO = 2 };                // the kernels' norm types
+enum { GN_F32 = NVDR_GRAD_F32, GN_BF16 = NVDR_GRAD_BF16, GN_F16 = NVDR_GRAD_F16 };
+
+struct GradTable {
+    uint64_t data[NVDR_GN_TENSORS];             // address, the type in the upper two bits
+    int64_t n[NVDR_GN_TENSORS];                 // elements, never zero
+    uint32_t first[NVDR_GN_TENSORS + 1];        // chunks in front of the tensor
+    float scale[NVDR_GN_TENSORS];
+    int n_tensors;
+};
+static_assert(sizeof(GradTable) <= 3900, "the kernel arguments have to fit 4 KB");
+
+typedef uint32_t gn_u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float gn_bf16(uint32_t bits) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ float gn_f16(uint32_t bits) { return (float)__builtin_bit_cast(_Float16, (unsigned short)bits); }
+
+// ---- one thread's sum ------------------------------------------------------------------------------------------------------------
+// p = infinity compares bit patterns: without the sign they order like the values, a NaN above infinity, so that a NaN survives.
+template <int P>
+struct GradSum {
+    double s = 0.0;
+    uint32_t m = 0;
+    __device__ __forceinline__ void add(float x)
+    {
+        if (P == GN_TWO) { const double d = (double)x; s = fma(d, d, s); }
+        else if (P == GN_ONE) s += fabs((double)x);
+        else m = max(m, __float_as_uint(x) & 0x7fffffffu);
+    }
+    template <int T>
+    __device__ __forceinline__ void add16(gn_u4 v)
+    {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (T == GN_F32) add(__uint_as_float(v[c]));
+            else if (T == GN_BF16) { add(gn_bf16(v[c] & 0xffffu)); add(__uint_as_float(v[c] & 0xffff0000u)); }
+            else { add(gn_f16(v[c] & 0xffffu)); add(gn_f16(v[c] >> 16)); }
+        }
+    }
+    __device__ __forceinline__ double value() const { return P == GN_INF ? (double)__uint_as_float(m) : s; }
+};
+
+template <int P>
+__device__ __forceinline__ double gn_join(double a, double b)
+{
+    if (P == GN_INF) return (a > b || a != a) ? a : b;
+    return a + b;
+}
+
+// the sum over the workgroup, in every thread; `lds`: one double per wavefront
+template <int P>
+__device__ __forceinline__ double gn_block_join(double v, double *lds)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = gn_join<P>(v, __shfl_xor(v, o));
+    __syncthreads();                                        // (a second call: the first one's values have been read)
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = gn_join<P>(v, lds[w]);
+    return v;
+}
+
+// ---- which part of which tensor ----------------------------------------------------------------------------------------------------
+// the tensor that chunk c falls into: the lanes compare 64 entries at a time (one round trip instead of a search's seven)
+__device__ __forceinline__ int gn_find(const GradTable &tab, uint32_t c)
+{
+    const int lane = threadIdx.x & 63;
+    int at = -1;
+    for (int q = 0; q < tab.n_tensors; q += 64)
+        at += __popcll(__ballot(q + lane < tab.n_tensors && tab.first[min(q + lane, NVDR_GN_TENSORS)] <= c));
+    return __builtin_amdgcn_readfirstlane(at);
+}
+
+// elements per chunk
+__device__ __forceinline__ int gn_chunk_len(int type) { return type == GN_F32 ? NVDR_GN_CHUNK / 4 : NVDR_GN_CHUNK / 2; }
+
+template <int P, int T>
+__device__ __forceinline__ double gn_sum_part(const char *p, int64_t count)
+{
+    constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE;
+    auto one = [&](int64_t i) -> float {
+        if (T == GN_F32) return ((const float *)p)[i];
+        const uint32_t h = ((const uint16_t *)p)[i];
+        return T == GN_BF16 ? gn_bf16(h) : gn_f16(h);
+    };
+    GradSum<P> a[4];
+    const int64_t head = min((int64_t)((16 - ((uintptr_t)p & 15)) & 15) / SIZE, count);     // up to the first 16-byte boundary
+    const int64_t nvec = (count - head) / VEC, tail = count - head - nvec * VEC;
+    if ((int64_t)threadIdx.x < head) a[0].add(one(threadIdx.x));
+    if ((int64_t)threadIdx.x < tail) a[1].add(one(head + nvec * VEC + threadIdx.x));
+    const gn_u4 *v = (const gn_u4 *)(p + head * SIZE);
+    int64_t i = threadIdx.x;
+    for (; i + 3 * NVDR_GN_BLOCK < nvec; i += 4 * NVDR_GN_BLOCK) {      // four loads in flight
+        gn_u4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = v[i + u * NVDR_GN_BLOCK];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a[u].template add16<T>(x[u]);
+    }
+    gn_u4 x[3];
+#pragma unroll
+    for (int u = 0; u < 3; ++u) x[u] = i + u * NVDR_GN_BLOCK < nvec ? v[i + u * NVDR_GN_BLOCK] : gn_u4{0, 0, 0, 0};     // (a zero adds nothing)
+#pragma unroll
+    for (int u = 0; u < 3; ++u) a[u].template add16<T>(x[u]);
+    return gn_join<P>(gn_join<P>(a[0].value(), a[1].value()), gn_join<P>(a[2].value(), a[3].value()));
+}
+
+template <int P>
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_part_kernel(GradTable tab, double *__restrict__ part)
+{
+    __shared__ double lds[NVDR_GN_BLOCK / 64];
+    const uint64_t chunks = tab.first[tab.n_tensors];
+    const uint32_t c1 = (uint32_t)((blockIdx.x + 1) * chunks / gridDim.x);
+    uint32_t c = (uint32_t)(blockIdx.x * chunks / gridDim.x);
+    double sum = 0.0;
+    for (int k = gn_find(tab, c); c < c1; ++k) {
+        const uint32_t first = tab.first[k], end = min(c1, tab.first[k + 1]);
+        const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
+        const char *p = (const char *)(tab.data[k] & ~(3ull << 62));
+        const int64_t e0 = (int64_t)(c - first) * len, e1 = min((int64_t)(end - first) * len, tab.n[k]);
+        double s;
+        if (type == GN_F32) s = gn_sum_part<P, GN_F32>(p + e0 * 4, e1 - e0);
+        else if (type == GN_BF16) s = gn_sum_part<P, GN_BF16>(p + e0 * 2, e1 - e0);
+        else s = gn_sum_part<P, GN_F16>(p + e0 * 2, e1 - e0);
+        const double w = fabs((double)tab.scale[k]);
+        sum = gn_join<P>(sum, P == GN_TWO ? s * (w * w) : s * w);
+        c = end;
+    }
+    sum = gn_block_join<P>(sum, lds);
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
+}
+
+// ---- the norm of the parts, and the factor -----------------------------------------------------------------------------------------
+template <int P>
+__device__ __forceinline__ double gn_total(const double *__restrict__ part, int n_part, double *lds)
+{
+    double v = 0.0;
+    for (int i = threadIdx.x; i < n_part; i += blockDim.x) v = gn_join<P>(v, part[i]);
+    v = gn_block_join<P>(v, lds);
+    return P == GN_TWO ? sqrt(v) : v;
+}
+
+// one rounding to fp32, of the quotient in fp64; a NaN stays a NaN.  An infinite max_norm never scales (inf / inf would)
+__device__ __forceinline__ float gn_factor(double norm, double max_norm)
+{
+    if (max_norm == (double)__builtin_inff()) return 1.0f;
+    const double f = max_norm / (norm + NVDR_GN_EPS);
+    return (float)(f > 1.0 ? 1.0 : f);
+}
+
+template <int P>
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_final_kernel(const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ out)
+{
+    __shared__ double lds[NVDR_GN_BLOCK / 64];
+    const double norm = gn_total<P>(part, n_part, lds);
+    if (threadIdx.x == 0) {
+        out[0] = (float)norm;
+        out[1] = gn_factor(norm, max_norm);
+    }
+}
+
+// ---- scaling -------------------------------------------------------------------------------------------------------------------------
+template <int T>
+__device__ __forceinline__ uint32_t gn_scaled(uint32_t w, float f)
+{
+    if (T == GN_F32) return __float_as_uint(__uint_as_float(w) * f);
+    if (T == GN_BF16) {
+        const uint32_t lo = __builtin_bit_cast(unsigned short, (__bf16)(gn_bf16(w & 0xffffu) * f));
+        return lo | ((uint32_t)__builtin_bit_cast(unsigned short, (__bf16)(__uint_as_float(w & 0xffff0000u) * f)) << 16);
+    }
+    const uint32_t lo = __builtin_bit_cast(unsigned short, (_Float16)(gn_f16(w & 0xffffu) * f));
+    return lo | ((uint32_t)__builtin_bit_cast(unsigned short, (_Float16)(gn_f16(w >> 16) * f)) << 16);
+}
+
+// from the end to the front: the norm's pass went the other way, and what it read last is still in the last-level cache
+template <int T>
+__device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
+{
+    constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE;
+    auto one = [&](int64_t i) {
+        if (T == GN_F32) ((float *)p)[i] *= f;
+        else ((uint16_t *)p)[i] = (uint16_t)gn_scaled<T>(((uint16_t *)p)[i], f);
+    };
+    const int64_t head = min((int64_t)((16 - ((uintptr_t)p & 15)) & 15) / SIZE, count);
+    const int64_t nvec = (count - head) / VEC, tail = count - head - nvec * VEC;
+    gn_u4 *v = (gn_u4 *)(p + head * SIZE);
+    for (int64_t b = (nvec + 4 * NVDR_GN_BLOCK - 1) / (4 * NVDR_GN_BLOCK) - 1; b >= 0; --b) {
+        const int64_t i = b * (4 * NVDR_GN_BLOCK) + threadIdx.x;
+        gn_u4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i + u * NVDR_GN_BLOCK < nvec) x[u] = v[i + u * NVDR_GN_BLOCK];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i + u * NVDR_GN_BLOCK >= nvec) break;
+            gn_u4 y;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = gn_scaled<T>(x[u][c], f);
+            v[i + u * NVDR_GN_BLOCK] = y;
+        }
+    }
+    if ((int64_t)threadIdx.x < head) one(threadIdx.x);
+    if ((int64_t)threadIdx.x < tail) one(head + nvec * VEC + threadIdx.x);
+}
+
+// n_part > 0: every workgroup adds the parts up itself, in the same order (a launch less than a kernel of its own for it), and the first one
+// writes the norm; n_part = 0: the factor is in out[1].
+template <int P>
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_scale_kernel(GradTable tab, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ out)
+{
+    __shared__ double lds[NVDR_GN_BLOCK / 64];
+    float f;
+    if (n_part > 0) {
+        const double norm = gn_total<P>(part, n_part, lds);
+        f = gn_factor(norm, max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            out[0] = (float)norm;
+            out[1] = f;
+        }
+    } else f = out[1];
+    if (f == 1.0f) return;
+    const uint64_t chunks = tab.first[tab.n_tensors];
+    const uint32_t c0 = (uint32_t)(blockIdx.x * chunks / gridDim.x);
+    uint32_t c = (uint32_t)((blockIdx.x + 1) * chunks / gridDim.x);
+    for (int k = c > c0 ? gn_find(tab, c - 1) : 0; c > c0; --k) {
+        const uint32_t first = tab.first[k], begin = max(c0, first);
+        const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
+        char *p = (char *)(tab.data[k] & ~(3ull << 62));
+        const int64_t e0 = (int64_t)(begin - first) * len, e1 = min((int64_t)(c - first) * len, tab.n[k]);
+        if (type == GN_F32) gn_scale_part<GN_F32>(p + e0 * 4, e1 - e0, f);
+        else if (type == GN_BF16) gn_scale_part<GN_BF16>(p + e0 * 2, e1 - e0, f);
+        else gn_scale_part<GN_F16>(p + e0 * 2, e1 - e0, f);
+        c = begin;
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+struct GradList {
+    const void *const *data;
+    const int64_t *n;
+    const uint8_t *type;
+    const float *scale;         // NULL: one
+    int64_t count;
+};
+
+static int64_t gn_size(int type) { return type == GN_F32 ? 4 : 2; }
+
+static int gn_check(const GradList &l, double max_norm, const double *workspace, int64_t workspace_len, const float *out, const char *who)
+{
+    NVDR_REQUIRE(l.count >= 0 && l.count < (1ll << 24), "%s: %lld tensors", who, (long long)l.count);
+    NVDR_REQUIRE(l.count == 0 || (l.data && l.n && l.type), "%s: NULL argument", who);
+    NVDR_REQUIRE(out && workspace && ((uintptr_t)workspace & 7) == 0, "%s: out and an 8-byte aligned workspace are needed", who);
+    NVDR_REQUIRE(workspace_len >= nvdr_grad_norm_workspace(l.count), "%s: a workspace of %lld doubles, %lld are needed", who, (long long)workspace_len,
+                 (long long)nvdr_grad_norm_workspace(l.count));
+    NVDR_REQUIRE(max_norm >= 0.0, "%s: max_norm has to be zero or more", who);       // (a NaN fails too)
+    for (int64_t k = 0; k < l.count; ++k) {
+        NVDR_REQUIRE(l.type[k] <= GN_F16, "%s: tensor %lld has type %d", who, (long long)k, (int)l.type[k]);
+        NVDR_REQUIRE(l.n[k] >= 0 && l.n[k] < (1ll << 42), "%s: tensor %lld has %lld elements", who, (long long)k, (long long)l.n[k]);
+        NVDR_REQUIRE(l.n[k] == 0 || (l.data[k] && (uintptr_t)l.data[k] < (1ull << 62)), "%s: tensor %lld has no memory", who, (long long)k);
+        NVDR_REQUIRE((uintptr_t)l.data[k] % (uintptr_t)gn_size(l.type[k]) == 0, "%s: tensor %lld is not aligned to its elements", who, (long long)k);
+    }
+    return 0;
+}
+
+// in place: no byte may belong to two tensors (two workgroups would scale it, or one read what the other has scaled)
+static int gn_check_apart(const GradList &l, const char *who)
+{
+    typedef std::pair<uintptr_t, uintptr_t> Span;
+    uintptr_t last = 0;
+    bool ordered = true;
+    for (int64_t k = 0; k < l.count && ordered; ++k) {
+        if (l.n[k] == 0) continue;
+        ordered = (uintptr_t)l.data[k] >= last;
+        last = (uintptr_t)l.data[k] + (uintptr_t)(l.n[k] * gn_size(l.type[k]));
+    }
+    if (ordered) return 0;
+    Span *s = (Span *)malloc(sizeof(Span) * (size_t)l.count);
+    NVDR_REQUIRE(s, "%s: out of host memory", who);
+    int64_t m = 0;
+    for (int64_t k = 0; k < l.count; ++k)
+        if (l.n[k]) s[m++] = Span((uintptr_t)l.data[k], (uintptr_t)l.data[k] + (uintptr_t)(l.n[k] * gn_size(l.type[k])));
+    std::sort(s, s + m);
+    bool apart = true;
+    for (int64_t k = 1; k < m; ++k) apart = apart && s[k].first >= s[k - 1].second;
+    free(s);
+    NVDR_REQUIRE(apart, "%s: two gradients share memory (the same tensor twice, or overlapping views)", who);
+    return 0;
+}
+
+// fills `tab` with tensors from *at on, moves *at behind them; returns the workgroups of the launch (0: nothing left)
+static unsigned gn_fill(const GradList &l, int64_t *at, GradTable &tab)
+{
+    int m = 0;
+    uint64_t chunks = 0;
+    tab.first[0] = 0;
+    while (*at < l.count) {
+        const int64_t k = *at, n = l.n[k];
+        const int type = l.type[k];
+        const uint64_t word = (uint64_t)(uintptr_t)l.data[k] | ((uint64_t)type << 62);
+        const float scale = l.scale ? l.scale[k] : 1.0f;
+        const int64_t len = NVDR_GN_CHUNK / gn_size(type);
+        if (n == 0) { ++*at; continue; }
+        if (m && tab.data[m - 1] + (uint64_t)(tab.n[m - 1] * gn_size(type)) == word && tab.scale[m - 1] == scale) {
+            // directly behind the one before, same type and scale: one tensor
+            const uint64_t c = (uint64_t)tab.first[m - 1] + (uint64_t)((tab.n[m - 1] + n + len - 1) / len);
+            if (c >= (1ull << 31)) break;
+            tab.n[m - 1] += n;
+            chunks = c;
+        } else {
+            const uint64_t c = chunks + (uint64_t)((n + len - 1) / len);
+            if (m == NVDR_GN_TENSORS || (m && c >= (1ull << 31))) break;
+            tab.data[m] = word; tab.n[m] = n; tab.scale[m] = scale;
+            ++m;
+            chunks = c;
+        }
+        tab.first[m] = (uint32_t)chunks;
+        ++*at;
+    }
+    tab.n_tensors = m;
+    return (unsigned)(chunks < NVDR_GN_GRID ? chunks : NVDR_GN_GRID);
+}
+
+extern "C" int64_t nvdr_grad_norm_workspace(int64_t n_tensors)
+{
+    // (a launch ends with the list or with a full table; the split by the number of chunks needs more than 2^31 of them, 32 TB)
+    return ((n_tensors + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID;
+}
+
+template <int P>
+static int gn_parts(const GradList &l, double *part, int *n_part, int *launches, hipStream_t st)
+{
+    GradTable tab;
+    int64_t at = 0;
+    *n_part = *launches = 0;
+    while (unsigned blocks = gn_fill(l, &at, tab)) {
+        grad_norm_part_kernel<P><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part + *n_part);
+        NVDR_LAUNCH_CHECK();
+        *n_part += (int)blocks;
+        ++*launches;
+    }
+    return 0;
+}
+
+template <int P>
+static int gn_norm(const GradList &l, double max_norm, double *part, float *out, hipStream_t st)
+{
+    int n_part, launches;
+    if (int r = gn_parts<P>(l, part, &n_part, &launches, st)) return r;
+    grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, n_part, max_norm, out);
+    NVDR_LAUNCH_CHECK();
+    return 0;
+}
+
+template <int P>
+static int gn_clip(const GradList &l, double max_norm, double *part, float *out, hipStream_t st)
+{
+    int n_part, launches;
+    if (int r = gn_parts<P>(l, part, &n_part, &launches, st)) return r;
+    if (launches != 1) {
+        grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, n_part, max_norm, out);
+        NVDR_LAUNCH_CHECK();
+        n_part = 0;
+    }
+    GradTable tab;
+    int64_t at = 0;
+    while (unsigned blocks = gn_fill(l, &at, tab)) {
+        grad_scale_kernel<P><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part, n_part, max_norm, out);
+        NVDR_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+extern "C" int nvdr_grad_norm(const void *const *data, const int64_t *n, const uint8_t *type, const float *scale, int64_t n_tensors, int norm_type, double max_norm,
+                              double *workspace, int64_t workspace_len, float *out, void *stream)
+{
+    NvdrRange range("nvdr_grad_norm");
+    const GradList l = {data, n, type, scale, n_tensors};
+    if (int r = gn_check(l, max_norm, workspace, workspace_len, out, "nvdr_grad_norm")) return r;
+    switch (norm_type) {
+    case NVDR_NORM_INF: return gn_norm<GN_INF>(l, max_norm, workspace, out, (hipStream_t)stream);
+    case NVDR_NORM_1: return gn_norm<GN_ONE>(l, max_norm, workspace, out, (hipStream_t)stream);
+    case NVDR_NORM_2: return gn_norm<GN_TWO>(l, max_norm, workspace, out, (hipStream_t)stream);
+    }
+    NVDR_REQUIRE(false, "nvdr_grad_norm: norm type %d", norm_type);
+}
+
+extern "C" int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t *type, int64_t n_tensors, int norm_type, double max_norm, double *workspace,
+                              int64_t workspace_len, float *out, void *stream)
+{
+    NvdrRange range("nvdr_grad_clip");
+    const GradList l = {(const void *const *)data, n, type, nullptr, n_tensors};
+    if (int r = gn_check(l, max_norm, workspace, workspace_len, out, "nvdr_grad_clip")) return r;
+    if (int r = gn_check_apart(l, "nvdr_grad_clip")) return r;
+    switch (norm_type) {
+    case NVDR_NORM_INF: return gn_clip<GN_INF>(l, max_norm, workspace, out, (hipStream_t)stream);
+    case NVDR_NORM_1: return gn_clip<GN_ONE>(l, max_norm, workspace, out, (hipStream_t)stream);
+    case NVDR_NORM_2: return gn_clip<GN_TWO>(l, max_norm, workspace, out, (hipStream_t)stream);
+    }
+    NVDR_REQUIRE(false, "nvdr_grad_clip: norm type %d", norm_type);
+}

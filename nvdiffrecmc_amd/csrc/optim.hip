@@ -20,7 +20,8 @@ struct AdamTable {
     int n;
 };
 
-__global__ void __launch_bounds__(256) adam_step_kernel(AdamTable tab, double lr, double beta1d, double beta2d, float eps, const int *state)
+__global__ void __launch_bounds__(256) adam_step_kernel(AdamTable tab, double lr, double beta1d, double beta2d, float eps, const int *state,
+                                                         const float *grad_factor)
 {
     // state[0] = steps taken so far, state[1] unused, then two doubles: beta1^step, beta2^step (kept as running products: pow() in
     // double costs a workgroup ~10 us of latency); read-only here, advanced by adam_advance_kernel behind this launch
@@ -29,6 +30,7 @@ __global__ void __launch_bounds__(256) adam_step_kernel(AdamTable tab, double lr
     // 0.001f, 1 - 0.999f is 1.3e-5 off (visible in the parameters after ten steps)
     const float beta2 = (float)beta2d, omb1 = (float)(1.0 - beta1d), omb2 = (float)(1.0 - beta2d);
     const int step = state[0] + 1;
+    const float factor = grad_factor ? *grad_factor : 1.0f;     // of clipping by the global norm (gradnorm.hip); times one changes no bit
     if (threadIdx.x == 0) {
         const double *pw = (const double *)(state + 2);
         const double b1p = (step == 1 ? 1.0 : pw[0]) * beta1d, b2p = (step == 1 ? 1.0 : pw[1]) * beta2d;
@@ -99,7 +101,7 @@ __global__ void __launch_bounds__(256) adam_step_kernel(AdamTable tab, double lr
 #pragma unroll
                 for (int c = 0; c < 3; ++c) {
                     const int64_t e = 3 * t + c;
-                    const float gg = g3[j0][c] * T.grad_scale, m0 = T.exp_avg[e], v0 = T.exp_avg_sq[e];
+                    const float gg = g3[j0][c] * T.grad_scale * factor, m0 = T.exp_avg[e], v0 = T.exp_avg_sq[e];
                     const float mm = m0 + (gg - m0) * omb1;
                     const float vv = v0 * beta2 + (omb2 * gg) * gg;
                     const float denom = sqrtf(vv) / bc2_sqrt + eps;
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(256) adam_step_kernel(AdamTable tab, double lr
 #pragma unroll
             for (int c = 0; c < 3; ++c) {
                 const int64_t e = 3 * t + c;
-                const float gg = T.grad[e] * T.grad_scale, m0 = T.exp_avg[e], v0 = T.exp_avg_sq[e];
+                const float gg = T.grad[e] * T.grad_scale * factor, m0 = T.exp_avg[e], v0 = T.exp_avg_sq[e];
                 const float mm = m0 + (gg - m0) * omb1;
                 const float vv = v0 * beta2 + (omb2 * gg) * gg;
                 const float denom = sqrtf(vv) / bc2_sqrt + eps;
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(256) adam_step_kernel(AdamTable tab, double lr
         for (int u = 0; u < 4; ++u) {
             if (!ok[u]) continue;
             const int64_t e = e0 + (int64_t)(j0 + u) * 256 + threadIdx.x;
-            const float gg = g[u] * T.grad_scale;
+            const float gg = g[u] * T.grad_scale * factor;
             const float mm = m[u] + (gg - m[u]) * omb1;                 // lerp_(grad, 1 - beta1)
             const float vv = v[u] * beta2 + (omb2 * gg) * gg;           // mul_(beta2).addcmul_(grad, grad, value = 1 - beta2)
             const float denom = sqrtf(vv) / bc2_sqrt + eps;
@@ -198,6 +200,12 @@ extern "C" int nvdr_adam_step(const nvdr_adam_tensor *tensors, int n_tensors, do
 extern "C" int nvdr_adam_step_partial(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps,
                                       int *state, int advance, void *stream_)
 {
+    return nvdr_adam_step_clipped(tensors, n_tensors, lr, beta1, beta2, eps, state, advance, nullptr, stream_);
+}
+
+extern "C" int nvdr_adam_step_clipped(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps,
+                                      int *state, int advance, const float *grad_factor, void *stream_)
+{
     NvdrRange range("nvdr_adam_step");
     NVDR_REQUIRE(tensors && state, "adam_step: NULL argument");
     NVDR_REQUIRE(n_tensors >= 1 && n_tensors <= NVDR_ADAM_MAX_TENSORS, "adam_step: %d tensors (1..%d supported)", n_tensors, NVDR_ADAM_MAX_TENSORS);
@@ -229,7 +237,7 @@ extern "C" int nvdr_adam_step_partial(const nvdr_adam_tensor *tensors, int n_ten
     }
     for (int k = n_tensors; k <= NVDR_ADAM_MAX_TENSORS; ++k) tab.first_block[k] = (int)blocks;
     if (blocks < 1) blocks = 1;
-    adam_step_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream_>>>(tab, lr, beta1, beta2, (float)eps, state);
+    adam_step_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream_>>>(tab, lr, beta1, beta2, (float)eps, state, grad_factor);
     if (advance) adam_advance_kernel<<<1, 1, 0, (hipStream_t)stream_>>>(state, beta1, beta2);
     NVDR_LAUNCH_CHECK();
     return 0;

@@ -1,15 +1,141 @@
-"""Adam + gradient scale + parameter clamps of one iteration in ONE kernel launch (csrc/optim.hip).
+"""Adam + gradient scale + parameter clamps of one iteration in ONE kernel launch (csrc/optim.hip), and the global norm of many gradient
+tensors with clipping by it (csrc/gradnorm.hip): on its own (grad_norm, clip_grad_norm_) or as part of the update (FusedAdam(max_norm=...)).
 
 Same update as torch.optim.Adam(params, lr, betas, eps) without weight decay / amsgrad (the optimizer of the reference,
 train.py:452-461), followed by the clamps the reference applies to its parameters after the step (train.py:470-476); the
 multiplication of the light gradient by 64 (train.py:439-440) enters as a per-tensor gradient scale.  The step counter lives in
 device memory, so the launch can be captured in a HIP graph.
 """
+import array
+import contextlib
 import math
 
 import torch
 
 from . import _lib
+
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # NVDR_GRAD_F32 / BF16 / F16
+_NORM_TYPES = {math.inf: 0, 1.0: 1, 2.0: 2}                                 # NVDR_NORM_INF / 1 / 2
+
+
+def _norm_code(norm_type):
+    code = _NORM_TYPES.get(float(norm_type))
+    if code is None:
+        raise ValueError('norm_type must be 1, 2 or inf (got %s)' % norm_type)
+    return code
+
+
+def _max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError('max_norm must be zero or more (got %s)' % max_norm)
+    return max_norm
+
+
+def _fills_its_memory(t):
+    """Whether the elements of `t` are distinct and lie without gaps, in whatever order (a permuted contiguous tensor)."""
+    need = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+class _GradList:
+    """The tensors of one call as the lists the library takes (host memory), checked: fp32 / bf16 / fp16 on one GPU.  A tensor whose
+    elements do not lie side by side (a slice) is replaced by a contiguous copy, kept in .copies as (index, copy)."""
+
+    def __init__(self, tensors, what, scales=None):
+        try:
+            where = {t.get_device() for t in tensors}
+            self.types = bytes([_GRAD_TYPES[t.dtype] for t in tensors])
+            plain = all([t.is_contiguous() for t in tensors])
+        except (AttributeError, KeyError, TypeError):
+            for t in tensors:
+                if not isinstance(t, torch.Tensor):
+                    raise TypeError('%s: gradients must be tensors (got %s)' % (what, type(t).__name__)) from None
+                if t.dtype not in _GRAD_TYPES:
+                    raise ValueError('%s: gradients must be float32, bfloat16 or float16 (got %s)' % (what, t.dtype)) from None
+            raise
+        if len(where) > 1 or -1 in where:
+            raise RuntimeError('%s: gradients must reside on one GPU; this path has no CPU fallback' % what)
+        self.copies = []
+        if not plain:
+            tensors = list(tensors)
+            for i, t in enumerate(tensors):
+                if t.layout is not torch.strided:
+                    raise ValueError('%s: gradients must be dense (got layout %s)' % (what, t.layout))
+                if not t.is_contiguous() and not _fills_its_memory(t):
+                    tensors[i] = t.contiguous()
+                    self.copies.append((i, tensors[i]))
+        self.tensors, self.count = tensors, len(tensors)
+        self._data = array.array('Q', [t.data_ptr() for t in tensors])
+        self._n = array.array('q', [t.numel() for t in tensors])
+        self._scales = None
+        if scales is not None:
+            self._scales = array.array('f', [float(s) for s in scales])
+            if len(self._scales) != self.count:
+                raise ValueError('%s: %d scales for %d tensors' % (what, len(self._scales), self.count))
+        self.data, self.n = self._data.buffer_info()[0], self._n.buffer_info()[0]
+        self.scales = self._scales.buffer_info()[0] if self._scales is not None else None
+
+
+def _on(device_index):
+    """Makes the device of the call's tensors the current one (launches go to the current device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
+
+
+def grad_norm(tensors, norm_type=2.0, scales=None):
+    """The norm of all `tensors` seen as one vector: (sum |scales[k] * g|^p)^(1/p) for norm_type p = 1 or 2, the largest magnitude for
+    math.inf; a NaN anywhere gives a NaN.  tensors: a tensor or an iterable of tensors, fp32 / bf16 / fp16 in any mixture and any layout,
+    on one GPU.  Returns a 0-d fp32 tensor on that GPU (0 on the CPU for an empty list); nothing waits for it.  Sums are kept in fp64."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    code = _norm_code(norm_type)
+    if not tensors:
+        return torch.zeros(())
+    lst = _GradList(tensors, 'grad_norm', scales)
+    lib, dev = _lib.load(), tensors[0].device
+    with _on(dev.index):
+        work = torch.empty(lib.nvdr_grad_norm_workspace(lst.count), dtype=torch.float64, device=dev)
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        _lib.check(lib.nvdr_grad_norm(lst.data, lst.n, lst.types, lst.scales, lst.count, code, math.inf, work.data_ptr(), work.numel(),
+                                      out.data_ptr(), _lib.stream_ptr()), 'grad_norm')
+    return out[0]
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns their norm BEFORE that (0-d fp32 on
+    the GPU): torch.nn.utils.clip_grad_norm_ with the norm kept in fp64 and two launches for up to 160 tensors (neighbours in memory, like
+    the views of a gradient bucket, count as one).  parameters: a tensor or an iterable; those without a gradient are left out.  A norm
+    that is infinite or NaN makes the gradients zero or NaN as it does there, unless error_if_nonfinite is set, which waits for the norm
+    and raises before anything is scaled (not inside a graph capture).  max_norm = inf only measures.  Gradients must not share memory."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros((), device=parameters[0].device if parameters else None)
+    if error_if_nonfinite:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('clip_grad_norm_: error_if_nonfinite reads the norm on the host, which a graph capture does not allow')
+        norm = grad_norm(grads, norm_type)
+        if not math.isfinite(norm.item()):
+            raise RuntimeError('clip_grad_norm_: the norm of the gradients is %s' % norm.item())
+    lst = _GradList(grads, 'clip_grad_norm_')
+    for i, _ in lst.copies:
+        if any(st == 0 and sz > 1 for st, sz in zip(grads[i].stride(), grads[i].shape)):
+            raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
+    lib, dev = _lib.load(), grads[0].device
+    with _on(dev.index):
+        work = torch.empty(lib.nvdr_grad_norm_workspace(lst.count), dtype=torch.float64, device=dev)
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        _lib.check(lib.nvdr_grad_clip(lst.data, lst.n, lst.types, lst.count, code, max_norm, work.data_ptr(), work.numel(),
+                                      out.data_ptr(), _lib.stream_ptr()), 'clip_grad_norm_')
+        with torch.no_grad():
+            for i, copy in lst.copies:
+                grads[i].copy_(copy)
+    torch.autograd.graph.increment_version(grads)
+    return out[0]
 
 
 class FusedAdam:
@@ -21,10 +147,13 @@ class FusedAdam:
     rates, train.py:336-356).  normalize3[i]: renormalise every texel of three channels after the clamps (the normal map).
     sparse[i]: the tensor is a three-channel texture whose gradient is zero almost everywhere (a nearest-texel lookup): tiles of 64
     texels without gradient and without history are skipped -- same parameters, a fraction of the traffic (csrc/optim.hip).
-    zero_grad[i] (with sparse): p.grad is zeroed behind the update (a persistent scatter-add buffer then needs no memset)."""
+    zero_grad[i] (with sparse): p.grad is zeroed behind the update (a persistent scatter-add buffer then needs no memset).
+    max_norm: the update sees its gradients -- with grad_scales and grad_mult -- scaled by min(1, max_norm / (norm + 1e-6)), norm =
+    the norm (norm_type 2, 1 or math.inf) of all tensors that are not frozen: clip_grad_norm_ in front of the step, without its pass over
+    the gradients, which stay as they are.  .grad_norm holds the norm of the last step (0-d, device; the next step overwrites it)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, clamps=None, grad_scales=None, lr_scales=None, normalize3=None,
-                 sparse=None, zero_grad=None):
+                 sparse=None, zero_grad=None, max_norm=None, norm_type=2.0):
         self.params = list(params)
         if not 1 <= len(self.params) <= 8:
             raise ValueError('FusedAdam: 1..8 parameter tensors')
@@ -41,11 +170,37 @@ class FusedAdam:
         self.active = [torch.zeros((p.numel() // 3 + 63) // 64, dtype=torch.uint8, device=p.device) if sp else None for p, sp in zip(self.params, self.sparse)]
         self.exp_avg = [torch.zeros_like(p) for p in self.params]
         self.exp_avg_sq = [torch.zeros_like(p) for p in self.params]
+        self.max_norm, self._norm_code = (None if max_norm is None else _max_norm(max_norm)), _norm_code(norm_type)
+        self._measured = False
+        dev = self.params[0].device
+        self._norm_out = torch.zeros(2, dtype=torch.float32, device=dev) if max_norm is not None else None       # norm, factor
+        self._norm_work = torch.empty(_lib.load().nvdr_grad_norm_workspace(len(self.params)), dtype=torch.float64, device=dev) if max_norm is not None else None
         self.state = torch.zeros(8, dtype=torch.int32, device=self.params[0].device)     # steps taken, scratch, beta1^t, beta2^t (doubles)
 
     @property
     def step_count(self):
         return int(self.state[0].item())
+
+    @property
+    def grad_norm(self):
+        """Norm of the gradients of the last step before clipping (0 before the first one; None without max_norm)."""
+        return None if self._norm_out is None else self._norm_out[0]
+
+    def measure_norm(self, grad_mult=1.0):
+        """The norm of this iteration's gradients into .grad_norm, and the factor of the updates that follow (max_norm).  step() calls it;
+        a caller that updates in subsets calls it once, when every gradient of the iteration is there, in front of the first subset."""
+        if self.max_norm is None:
+            raise RuntimeError('FusedAdam.measure_norm: no max_norm was given')
+        live = [i for i in range(len(self.params)) if float(self.lr_scales[i]) != 0.0]
+        for i in live:
+            if self.params[i].grad is None:
+                raise RuntimeError('FusedAdam.step: parameter %d has no gradient' % i)
+        lst = _GradList([self.params[i].grad for i in live], 'FusedAdam', [float(self.grad_scales[i]) * float(grad_mult) for i in live])
+        lib, dev = _lib.load(), self.params[0].device
+        with _on(dev.index):
+            _lib.check(lib.nvdr_grad_norm(lst.data, lst.n, lst.types, lst.scales, lst.count, self._norm_code, self.max_norm, self._norm_work.data_ptr(),
+                                          self._norm_work.numel(), self._norm_out.data_ptr(), _lib.stream_ptr()), 'grad_norm')
+        self._measured = True
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -57,7 +212,16 @@ class FusedAdam:
     def step(self, subset=None, advance=True, grad_mult=1.0):
         """subset: indices of the tensors to update in this launch (None = all); advance=False leaves the step counter alone (every
         launch of an iteration but the last, nvdr_adam_step_partial); grad_mult: extra factor on the gradients of this launch (1 / world
-        after a summing all-reduce)."""
+        after a summing all-reduce).  With max_norm a launch of all tensors measures the norm first; subsets need measure_norm() before the
+        first of them."""
+        factor = None
+        if self.max_norm is not None:
+            if subset is None:
+                self.measure_norm(grad_mult)
+            elif not self._measured:
+                raise RuntimeError('FusedAdam.step: with max_norm, measure_norm() comes before the first subset of an iteration')
+            factor = self._norm_out.data_ptr() + 4
+            self._measured = not advance
         idx = list(range(len(self.params))) if subset is None else list(subset)
         tab = (_lib.NvdrAdamTensor * len(idx))()
         keep = []
@@ -90,6 +254,6 @@ class FusedAdam:
             t.frozen = int(float(self.lr_scales[i]) == 0.0)
             t.active = self.active[i].data_ptr() if self.active[i] is not None else None
             t.zero_grad = int(bool(self.zero_grad_after[i] and self.active[i] is not None))
-        with torch.no_grad():
-            _lib.check(_lib.load().nvdr_adam_step_partial(tab, len(idx), self.lr, self.betas[0], self.betas[1], self.eps,
-                                                          _lib.ptr(self.state), int(bool(advance)), _lib.stream_ptr()), 'adam_step')
+        with torch.no_grad(), _on(self.state.get_device()):
+            _lib.check(_lib.load().nvdr_adam_step_clipped(tab, len(idx), self.lr, self.betas[0], self.betas[1], self.eps,
+                                                          _lib.ptr(self.state), int(bool(advance)), factor, _lib.stream_ptr()), 'adam_step')

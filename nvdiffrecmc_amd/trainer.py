@@ -40,7 +40,7 @@ from . import renderutils as ru
 from . import scene as sc
 from .denoiser import BilateralDenoiser, _safe_normalize
 from .light import EnvironmentLight
-from .optim import FusedAdam
+from .optim import FusedAdam, clip_grad_norm_
 from . import mesh as mesh_ops
 from . import render as rd
 from . import _lib
@@ -119,7 +119,8 @@ class DirectLightingStep:
                  probe_res=256, denoise=True, retrace_backward=False, pixel_index_offset=0, subdiv=0, lr=0.01, fused=True,
                  denoiser_demodulate=True, light_grad_scale=64.0, use_graph=False, material_set='full', tex_res=1024,
                  optimize_geometry=False, lr_pos=None, lr_light=None, perturb_pos=0.0, ks_min=(0.0, 0.08, 0.0), ks_max=(0.0, 1.0, 1.0),
-                 perturbed_nrm=True, exchange_mode='dense', pipeline=True, force_exchange=False, union_views=None, build_mode=None, rebuild_every=1):
+                 perturbed_nrm=True, exchange_mode='dense', pipeline=True, force_exchange=False, union_views=None, build_mode=None, rebuild_every=1,
+                 max_grad_norm=None):
         self.dev = torch.device(device)
         self.res, self.n, self.view = res, n_samples_x, view     # view: an index or a list of indices (a batch of views)
         self.pixel_index_offset = pixel_index_offset
@@ -147,6 +148,11 @@ class DirectLightingStep:
         # rebuild=1 every iteration) and the default.  Locked geometry is rebuilt every iteration whatever K (as the reference does).
         self.rebuild_every = max(1, int(rebuild_every))
         self._iter = 0
+        # max_grad_norm: the gradients of all trained tensors -- the light's with its factor of 64, summed over the ranks and averaged -- are scaled
+        # by min(1, max_grad_norm / (norm + 1e-6)) in front of Adam (optim.FusedAdam(max_norm=...); the reference does not clip): a view whose
+        # estimate has an outlier moves the parameters no further than another.  None = no clipping.  With several ranks every update then
+        # waits for the last chunk of the exchange, since the norm is over all of them.
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
         # union_views (with force_exchange): the views of the WHOLE batch; the tile flags of this one rank are OR-ed with the tiles those views
         # touch, so that the one-rank run compacts, sends and scatters the bytes the several-rank run would (bench.py one_view)
         self._union_views = list(union_views) if (union_views is not None and force_exchange) else None
@@ -281,7 +287,7 @@ class DirectLightingStep:
         if self._fused_update:
             sparse = [nm in ('kd', 'ks', 'normal') and material_set == 'full' for nm in names]
             self.opt = FusedAdam(self.params, lr=lr, grad_scales=grad_scales, clamps=clamps, lr_scales=lr_scales, normalize3=norm3,
-                                 sparse=sparse, zero_grad=sparse)
+                                 sparse=sparse, zero_grad=sparse, max_norm=self.max_grad_norm)
             if material_set == 'full':
                 self._tex_grad = rd.PersistentGrads(torch.zeros_like(p) for p in self.params[:self.n_tex])
         else:
@@ -557,6 +563,8 @@ class DirectLightingStep:
                     p.grad.mul_(grad_mult)
         if self.light.base.grad is not None and self.light_grad_scale != 1.0:
             self.light.base.grad *= self.light_grad_scale       # train.py:439-440
+        if self.max_grad_norm is not None:
+            clip_grad_norm_([p for p, k in zip(self.params, self._lr_scales) if k != 0.0], self.max_grad_norm)
         self.opt.step()
         with torch.no_grad():
             self.kd_tex.clamp_(0.0, 1.0)
@@ -723,12 +731,21 @@ class DirectLightingStep:
             self._packed_tex_grad()
             ex.compute_flags()
         ex.start(skip_single=not self.force_exchange)
-        for k in range(last):                       # the early chunks: their update, then the next iteration's geometry stage can go
-            f = self._wait(k)
+        clip = self._fused_update and self.max_grad_norm is not None
+        if clip:                                    # the norm is over every chunk: all of them arrive, then all of them are updated
+            for k in range(last + 1):
+                f = self._wait(k)
+            if graphs:
+                self._graph_norm.replay()
+            else:
+                self.opt.measure_norm(f)
+        for k in range(last + 1 if clip else last):  # the early chunks: their update, then the next iteration's geometry stage can go
+            if not clip:
+                f = self._wait(k)
             if graphs:
                 gb[k].replay()
             else:
-                self._update(subset=chunks[k], advance=False, grad_mult=f)
+                self._update(subset=chunks[k], advance=(k == last), grad_mult=f)
         if self.pipeline and last > 0:
             if self.measure_exposed:        # how long the geometry stage keeps the main stream busy: what the texture chunk's wire time hides behind
                 a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -741,6 +758,9 @@ class DirectLightingStep:
             if self.measure_exposed:
                 b.record()
                 self._stage1_events.append((a, b))
+        if clip:
+            self.allreduce_bytes = ex.bytes_per_step
+            return loss
         ex.send(last)                               # sparse: the host reads the union's size here -- the GPU is busy with stage 1 meanwhile
         self._pending = True
         if not (self.pipeline and last > 0):
@@ -911,6 +931,14 @@ class DirectLightingStep:
         # trained geometry the tensors G1's autograd graph saved must survive from G1 to G2's backward -- B_1 replays in between and must
         # not be handed their memory.  (The fused update allocates nothing today: asserted below, so that a change of it is noticed.)
         pool_b = None
+        if self._fused_update and self.max_grad_norm is not None:
+            # the norm over all chunks, replayed when the last one has arrived and in front of the first update
+            for k in range(n):
+                f = self._point_grads(k)
+            self._graph_norm = torch.cuda.CUDAGraph()
+            with _capture_graph(self._graph_norm):
+                self.opt.measure_norm(f)
+            pool_b = self._graph_norm.pool()
         for k in range(n):
             f = self._point_grads(k)        # the .grad of chunk k = views into its bucket: what the captured update reads on every replay
             gk = torch.cuda.CUDAGraph()

@@ -1,0 +1,110 @@
+"""What the gradient norm, the clipping and the clipped Adam step refuse, and what they do without a launch (no GPU needed)."""
+import array
+import ctypes
+import math
+
+import pytest
+import torch
+
+from nvdiffrecmc_amd import _lib, optim
+
+
+def _param(grad):
+    p = torch.nn.Parameter(torch.zeros(grad.shape, dtype=grad.dtype))
+    p.grad = grad
+    return p
+
+
+def test_python_refusals():
+    x = torch.zeros(3)
+    for call in (lambda t, **k: optim.grad_norm([t], **k), lambda t, **k: optim.clip_grad_norm_([_param(t)], 1.0, **k)):
+        with pytest.raises(RuntimeError, match='GPU'):
+            call(x)
+        with pytest.raises(ValueError, match='float64'):
+            call(x.double())
+        for p in (0.0, 3.0, -math.inf, math.nan):
+            with pytest.raises(ValueError, match='norm_type'):
+                call(x, norm_type=p)
+    with pytest.raises(TypeError, match='float'):
+        optim.grad_norm([1.0])
+    with pytest.raises(RuntimeError):
+        optim.grad_norm([torch.eye(3).to_sparse()])
+    for m in (-1.0, math.nan, -math.inf):
+        with pytest.raises(ValueError, match='max_norm'):
+            optim.clip_grad_norm_([_param(x)], m)
+
+
+def test_nothing_to_do():
+    assert optim.grad_norm([]).item() == 0.0
+    assert optim.clip_grad_norm_([], 1.0).item() == 0.0
+    assert optim.clip_grad_norm_([torch.nn.Parameter(torch.ones(3))], 1.0).item() == 0.0          # no gradient
+    assert optim.clip_grad_norm_(torch.nn.Parameter(torch.ones(3)), 1.0).item() == 0.0
+    assert optim.clip_grad_norm_((p for p in ()), 1.0).item() == 0.0
+
+
+def test_permuted_and_sliced_layouts_are_told_apart():
+    x = torch.zeros(4, 5, 6)
+    for t, want in ((x, True), (x.permute(2, 0, 1), True), (x.transpose(0, 2), True), (x[:, :, :3], False), (x[::2], False), (x[:1], True),
+                    (torch.zeros(1).expand(7), False), (x.permute(1, 0, 2)[:2], False), (x[:, :1].transpose(0, 1), False), (torch.zeros(()), True)):
+        assert optim._fills_its_memory(t) == want, (t.shape, t.stride())
+
+
+# ---- the C entries refuse before anything is launched -----------------------------------------------------------------------------------
+
+def _call(entry, data, n, types, max_norm=1.0, norm_type=2, workspace=None, out=True, scale=None):
+    """The entry on host lists (addresses are never dereferenced: every call here is refused)."""
+    lib = _lib.load()
+    d, c = array.array('Q', data), array.array('q', n)
+    need = lib.nvdr_grad_norm_workspace(len(n))
+    ws = torch.empty(need if workspace is None else workspace, dtype=torch.float64)
+    o = torch.empty(2)
+    args = [d.buffer_info()[0], c.buffer_info()[0], bytes(types)] + ([scale] if entry == 'nvdr_grad_norm' else [])
+    args += [len(n), norm_type, max_norm, ws.data_ptr(), ws.numel(), o.data_ptr() if out else None, None]
+    rc = getattr(lib, entry)(*args)
+    return rc, (lib.nvdr_last_error() or b'').decode()
+
+
+@pytest.mark.parametrize('entry', ['nvdr_grad_norm', 'nvdr_grad_clip'])
+def test_entries_refuse_bad_arguments(entry):
+    A = 1 << 20
+    cases = [
+        (dict(data=[A], n=[4], types=[3]), 'type'),
+        (dict(data=[A], n=[-1], types=[0]), 'elements'),
+        (dict(data=[A], n=[1 << 42], types=[0]), 'elements'),
+        (dict(data=[0], n=[4], types=[0]), 'no memory'),
+        (dict(data=[A + 2], n=[4], types=[0]), 'aligned'),
+        (dict(data=[A + 1], n=[4], types=[1]), 'aligned'),
+        (dict(data=[A], n=[4], types=[0], workspace=8), 'workspace'),
+        (dict(data=[A], n=[4], types=[0], out=False), 'out'),
+        (dict(data=[A], n=[4], types=[0], max_norm=-1.0), 'max_norm'),
+        (dict(data=[A], n=[4], types=[0], max_norm=math.nan), 'max_norm'),
+        (dict(data=[A], n=[4], types=[0], norm_type=3), 'norm type'),
+        (dict(data=[A], n=[4], types=[0], norm_type=-1), 'norm type'),
+    ]
+    for kw, word in cases:
+        rc, msg = _call(entry, **kw)
+        assert rc == -1 and word in msg, (kw, rc, msg)
+    lib = _lib.load()
+    ws, o = torch.empty(8192, dtype=torch.float64), torch.empty(2)
+    tail = [2, 1.0, ws.data_ptr(), ws.numel(), o.data_ptr(), None]
+    assert getattr(lib, entry)(*([None, None, None] + ([None] if entry == 'nvdr_grad_norm' else []) + [1] + tail)) == -1
+    assert getattr(lib, entry)(*([None, None, None] + ([None] if entry == 'nvdr_grad_norm' else []) + [-1] + tail)) == -1
+
+
+def test_clip_refuses_gradients_that_share_memory():
+    A = 1 << 20
+    for data, n, types in (([A, A], [4, 4], [0, 0]), ([A + 64, A], [4, 17], [0, 0]), ([A, A + 8], [4, 4], [0, 0]), ([A + 4096, A + 6, A], [8, 8, 4], [0, 1, 1])):
+        rc, msg = _call('nvdr_grad_clip', data, n, types)
+        assert rc == -1 and 'share memory' in msg, (data, n, rc, msg)
+
+
+def test_workspace_grows_with_the_list():
+    lib = _lib.load()
+    sizes = [lib.nvdr_grad_norm_workspace(n) for n in (0, 1, 160, 161, 1000)]
+    assert sizes[0] > 0 and sizes == sorted(sizes) and sizes[1] == sizes[2] < sizes[3] < sizes[4]
+
+
+def test_adam_entry_refuses_without_a_launch():
+    lib = _lib.load()
+    rc = lib.nvdr_adam_step_clipped(None, 0, ctypes.c_double(1e-3), 0.9, 0.999, 1e-8, None, 1, None, None)
+    assert rc == -1 and b'NULL' in lib.nvdr_last_error()

@@ -498,16 +498,16 @@ int nvdr_adam_step_clipped(const nvdr_adam_tensor *tensors, int n_tensors, doubl
  * data[k]: n[k] contiguous elements of type[k] in any mixture, aligned to their own size; n[k] = 0 is skipped.  scale: NULL for ones.  The
  * four lists live in HOST memory and are read before the call returns (a captured graph keeps them).  Sums in fp64, in an order that depends
  * on sizes and alignment only.  workspace: nvdr_grad_norm_workspace(n_tensors) doubles of device memory, nothing to initialise; launches that
- * may run at the same time need one each.  out[0] = norm, out[1] = factor (fp32, device).
+ * may run at the same time need one each.  norm, factor: one float each in device memory (factor may be NULL).
  * nvdr_grad_norm leaves the gradients alone; nvdr_grad_clip multiplies them by the factor in place (computed in fp32, one rounding to the
  * element's type) and writes nothing when the factor is one.  Gradients of nvdr_grad_clip must not share memory. */
 enum { NVDR_GRAD_F32 = 0, NVDR_GRAD_BF16 = 1, NVDR_GRAD_F16 = 2 };
 enum { NVDR_NORM_INF = 0, NVDR_NORM_1 = 1, NVDR_NORM_2 = 2 };
 int64_t nvdr_grad_norm_workspace(int64_t n_tensors);
 int nvdr_grad_norm(const void *const *data, const int64_t *n, const uint8_t *type, const float *scale, int64_t n_tensors, int norm_type,
-                   double max_norm, double *workspace, int64_t workspace_len, float *out, void *stream);
+                   double max_norm, double *workspace, int64_t workspace_len, float *norm, float *factor, void *stream);
 int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t *type, int64_t n_tensors, int norm_type, double max_norm,
-                   double *workspace, int64_t workspace_len, float *out, void *stream);
+                   double *workspace, int64_t workspace_len, float *norm, void *stream);
 
 /* ---- tile-sparse gradient exchange (additive; the reference has no distributed code).  The data-parallel step all-reduces the
  * gradients of the trained textures; with nearest-texel lookups they are zero outside the tiles (tile_floats contiguous floats, e.g.

@@ -6,6 +6,7 @@ render/renderutils/ops.py:78-83).  There is NO fallback: if the HIP library is m
 call fails, a RuntimeError is raised.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch  # noqa: F401  (must be imported first: maps the HIP runtime the library binds to)
@@ -174,8 +175,8 @@ _SIGNATURES = {
     'nvdr_adam_step_partial': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p],
     'nvdr_adam_step_clipped': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p, c_void_p],
     'nvdr_grad_norm_workspace': [c_int64],
-    'nvdr_grad_norm': [c_void_p, c_void_p, ctypes.c_char_p, c_void_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
-    'nvdr_grad_clip': [c_void_p, c_void_p, ctypes.c_char_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
+    'nvdr_grad_norm': [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, c_void_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
+    'nvdr_grad_clip': [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
     'nvdr_abi_sizeof': [c_int],
     'nvdr_tile_flags': [c_void_p, c_int64, c_int, c_void_p, c_void_p],
     'nvdr_tile_plan': [c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
@@ -228,6 +229,22 @@ def load():
                                '(__graft_entry__.build()) or update nvdiffrecmc_amd/_lib.py' % (mirror, want, have))
     _lib = lib
     return lib
+
+
+_gradlist = None
+
+
+def gradlist():
+    """The extension that reads lists of gradients (csrc/gradlist.cpp).  Raises RuntimeError when it is not built."""
+    global _gradlist
+    if _gradlist is None:
+        path = _build.GRADLIST
+        if not os.path.exists(path):
+            raise RuntimeError("_gradlist.so is not built (%s). Build it first: python -c 'import __graft_entry__ as g; g.build()'" % path)
+        spec = importlib.util.spec_from_file_location('_gradlist', path)
+        _gradlist = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_gradlist)
+    return _gradlist
 
 
 def check(rc, what):

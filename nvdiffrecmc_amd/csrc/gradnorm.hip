@@ -12,20 +12,37 @@
 // workgroup writes its sum to a place of its own and they are added in a fixed order, so that a result depends on the values, the sizes
 // and the alignment alone.
 //
-// Work split.  The tensors are cut into chunks of NVDR_GN_CHUNK bytes; a launch has at most NVDR_GN_GRID workgroups, each of which takes a
-// contiguous run of chunks, whatever tensors they fall into: a long tensor is shared by many workgroups and many short ones by few.  The table
-// of the tensors travels in the kernel arguments -- by value, so that a captured graph keeps it and no copy to the device is needed -- which
-// bounds the tensors of a launch; longer lists take several launches.  Neighbours in memory (views of one bucket) become one entry.
+// Work split.  The tensors are cut into chunks of NVDR_GN_CHUNK bytes, and runs of chunks, whatever tensors they fall into, are dealt to the
+// workgroups in turn, as many rounds of equally long runs as NVDR_GN_RUN gives: a long tensor is shared by many workgroups, many short ones
+// by few, and no workgroup has more than one run more than another.  The table of the tensors travels in the kernel arguments -- by value, so
+// that a captured graph keeps it and no copy to the device is needed -- which bounds the tensors of a launch; longer lists take several
+// launches.  Neighbours in memory (views of one bucket) become one entry.
+//
+// What was measured (us a call on MI355X; 789 M fp32 = 3.16 GB | 296 M bf16 = 0.59 GB in 315 tensors | 10.7 M fp32 = 43 MB in the cache):
+//   norm   one contiguous run per workgroup, plain loads          515 | 104 | 12.4
+//          the same with non-temporal loads                       458 |  92 | 12.5
+//          runs of 128 KB dealt in turn, non-temporal             449 |  96 | 12.4      (7.0 TB/s; 32 KB runs: 468 | 132 | 13.2)
+//   clip   one contiguous run per workgroup, plain               1783 | 357 | 23.4
+//          the last 160 MB of the norm's pass loaded to stay,
+//          the scaling from the end to the front, non-temporal   1675 | 307 | 23.4
+//          runs of 128 KB dealt in turn                          1581 | 300 | 23.3
+//          scaling by 256 workgroups of 1024, eight loads deep   1472 | 293 | 24.7      (6.2 TB/s of reading and writing)
+// A list that fits the last-level cache is left there: plain loads and stores (non-temporal ones cost 29 instead of 23 us at 43 MB), for the
+// scaling and for whoever reads the gradients next.
 #include <stdlib.h>
 #include <algorithm>
 
 #include "common.h"
 #include "nvdr_hip.h"
 
-#define NVDR_GN_BLOCK 512
-#define NVDR_GN_GRID 1024
-#define NVDR_GN_TENSORS 160
-#define NVDR_GN_CHUNK 16384
+#define NVDR_GN_BLOCK 512               // threads of a workgroup of the norm, and of the scaling of a list that fits the cache
+#define NVDR_GN_GRID 512                // workgroups of a launch at most: two per CU
+#define NVDR_GN_STREAM_BLOCK 1024       // the scaling of a longer list: fewer places in memory at a time
+#define NVDR_GN_STREAM_GRID 256
+#define NVDR_GN_TENSORS 160             // of a launch: the kernel arguments end at 4 KB
+#define NVDR_GN_CHUNK 4096              // bytes
+#define NVDR_GN_RUN (128 << 10)         // bytes
+#define NVDR_GN_KEEP (160ll << 20)      // bytes that stay in the last-level cache (256 MB) from one pass to the next: 96 to 256 MB within 2 %
 #define NVDR_GN_EPS 1e-6
 
 enum { GN_INF = 0, GN_ONE = 1, GN_TWO = 2 };                // the kernels' norm types
@@ -37,6 +54,8 @@ struct GradTable {
     uint32_t first[NVDR_GN_TENSORS + 1];        // chunks in front of the tensor
     float scale[NVDR_GN_TENSORS];
     int n_tensors;
+    uint32_t run;                               // chunks that a workgroup takes at a time
+    uint32_t kept;                              // chunks from here on are loaded to stay in the last-level cache
 };
 static_assert(sizeof(GradTable) <= 3900, "the kernel arguments have to fit 4 KB");
 
@@ -105,7 +124,10 @@ __device__ __forceinline__ int gn_find(const GradTable &tab, uint32_t c)
 // elements per chunk
 __device__ __forceinline__ int gn_chunk_len(int type) { return type == GN_F32 ? NVDR_GN_CHUNK / 4 : NVDR_GN_CHUNK / 2; }
 
-template <int P, int T>
+template <bool NT>
+__device__ __forceinline__ gn_u4 gn_load(const gn_u4 *p) { return NT ? __builtin_nontemporal_load(p) : *p; }
+
+template <int P, int T, bool NT>
 __device__ __forceinline__ double gn_sum_part(const char *p, int64_t count)
 {
     constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE;
@@ -124,38 +146,48 @@ __device__ __forceinline__ double gn_sum_part(const char *p, int64_t count)
     for (; i + 3 * NVDR_GN_BLOCK < nvec; i += 4 * NVDR_GN_BLOCK) {      // four loads in flight
         gn_u4 x[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = v[i + u * NVDR_GN_BLOCK];
+        for (int u = 0; u < 4; ++u) x[u] = gn_load<NT>(v + i + u * NVDR_GN_BLOCK);
 #pragma unroll
         for (int u = 0; u < 4; ++u) a[u].template add16<T>(x[u]);
     }
     gn_u4 x[3];
 #pragma unroll
-    for (int u = 0; u < 3; ++u) x[u] = i + u * NVDR_GN_BLOCK < nvec ? v[i + u * NVDR_GN_BLOCK] : gn_u4{0, 0, 0, 0};     // (a zero adds nothing)
+    for (int u = 0; u < 3; ++u) x[u] = i + u * NVDR_GN_BLOCK < nvec ? gn_load<NT>(v + i + u * NVDR_GN_BLOCK) : gn_u4{0, 0, 0, 0};     // (a zero adds nothing)
 #pragma unroll
     for (int u = 0; u < 3; ++u) a[u].template add16<T>(x[u]);
     return gn_join<P>(gn_join<P>(a[0].value(), a[1].value()), gn_join<P>(a[2].value(), a[3].value()));
+}
+
+template <int P, bool NT>
+__device__ __forceinline__ double gn_sum_typed(const char *p, int type, int64_t e0, int64_t e1)
+{
+    if (type == GN_F32) return gn_sum_part<P, GN_F32, NT>(p + e0 * 4, e1 - e0);
+    if (type == GN_BF16) return gn_sum_part<P, GN_BF16, NT>(p + e0 * 2, e1 - e0);
+    return gn_sum_part<P, GN_F16, NT>(p + e0 * 2, e1 - e0);
 }
 
 template <int P>
 __global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_part_kernel(GradTable tab, double *__restrict__ part)
 {
     __shared__ double lds[NVDR_GN_BLOCK / 64];
-    const uint64_t chunks = tab.first[tab.n_tensors];
-    const uint32_t c1 = (uint32_t)((blockIdx.x + 1) * chunks / gridDim.x);
-    uint32_t c = (uint32_t)(blockIdx.x * chunks / gridDim.x);
+    const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, kept = tab.kept;
     double sum = 0.0;
-    for (int k = gn_find(tab, c); c < c1; ++k) {
-        const uint32_t first = tab.first[k], end = min(c1, tab.first[k + 1]);
-        const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
-        const char *p = (const char *)(tab.data[k] & ~(3ull << 62));
-        const int64_t e0 = (int64_t)(c - first) * len, e1 = min((int64_t)(end - first) * len, tab.n[k]);
-        double s;
-        if (type == GN_F32) s = gn_sum_part<P, GN_F32>(p + e0 * 4, e1 - e0);
-        else if (type == GN_BF16) s = gn_sum_part<P, GN_BF16>(p + e0 * 2, e1 - e0);
-        else s = gn_sum_part<P, GN_F16>(p + e0 * 2, e1 - e0);
-        const double w = fabs((double)tab.scale[k]);
-        sum = gn_join<P>(sum, P == GN_TWO ? s * (w * w) : s * w);
-        c = end;
+    for (uint64_t r = (uint64_t)blockIdx.x * run; r < chunks; r += (uint64_t)gridDim.x * run) {
+        uint32_t c = (uint32_t)r;
+        const uint32_t c1 = min(c + run, chunks);
+        int k = gn_find(tab, c);
+        while (c < c1) {
+            const bool stream = c < kept;
+            const uint32_t first = tab.first[k], next = tab.first[k + 1], end = min(stream ? min(kept, c1) : c1, next);
+            const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
+            const char *p = (const char *)(tab.data[k] & ~(3ull << 62));
+            const int64_t e0 = (int64_t)(c - first) * len, e1 = min((int64_t)(end - first) * len, tab.n[k]);
+            const double s = stream ? gn_sum_typed<P, true>(p, type, e0, e1) : gn_sum_typed<P, false>(p, type, e0, e1);
+            const double w = fabs((double)tab.scale[k]);
+            sum = gn_join<P>(sum, P == GN_TWO ? s * (w * w) : s * w);
+            c = end;
+            k += end == next;
+        }
     }
     sum = gn_block_join<P>(sum, lds);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -180,13 +212,13 @@ __device__ __forceinline__ float gn_factor(double norm, double max_norm)
 }
 
 template <int P>
-__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_final_kernel(const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ out)
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_final_kernel(const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm, float *__restrict__ factor)
 {
     __shared__ double lds[NVDR_GN_BLOCK / 64];
-    const double norm = gn_total<P>(part, n_part, lds);
+    const double v = gn_total<P>(part, n_part, lds);
     if (threadIdx.x == 0) {
-        out[0] = (float)norm;
-        out[1] = gn_factor(norm, max_norm);
+        *norm = (float)v;
+        if (factor) *factor = gn_factor(v, max_norm);
     }
 }
 
@@ -204,10 +236,10 @@ __device__ __forceinline__ uint32_t gn_scaled(uint32_t w, float f)
 }
 
 // from the end to the front: the norm's pass went the other way, and what it read last is still in the last-level cache
-template <int T>
+template <int T, bool NT>
 __device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
 {
-    constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE;
+    constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE, BLOCK = NT ? NVDR_GN_STREAM_BLOCK : NVDR_GN_BLOCK, DEEP = NT ? 8 : 4;
     auto one = [&](int64_t i) {
         if (T == GN_F32) ((float *)p)[i] *= f;
         else ((uint16_t *)p)[i] = (uint16_t)gn_scaled<T>(((uint16_t *)p)[i], f);
@@ -215,19 +247,20 @@ __device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
     const int64_t head = min((int64_t)((16 - ((uintptr_t)p & 15)) & 15) / SIZE, count);
     const int64_t nvec = (count - head) / VEC, tail = count - head - nvec * VEC;
     gn_u4 *v = (gn_u4 *)(p + head * SIZE);
-    for (int64_t b = (nvec + 4 * NVDR_GN_BLOCK - 1) / (4 * NVDR_GN_BLOCK) - 1; b >= 0; --b) {
-        const int64_t i = b * (4 * NVDR_GN_BLOCK) + threadIdx.x;
-        gn_u4 x[4];
+    for (int64_t b = (nvec + DEEP * BLOCK - 1) / (DEEP * BLOCK) - 1; b >= 0; --b) {
+        const int64_t i = b * (DEEP * BLOCK) + threadIdx.x;
+        gn_u4 x[DEEP];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i + u * NVDR_GN_BLOCK < nvec) x[u] = v[i + u * NVDR_GN_BLOCK];
+        for (int u = 0; u < DEEP; ++u)
+            if (i + u * BLOCK < nvec) x[u] = gn_load<NT>(v + i + u * BLOCK);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (i + u * NVDR_GN_BLOCK >= nvec) break;
+        for (int u = 0; u < DEEP; ++u) {
+            if (i + u * BLOCK >= nvec) break;
             gn_u4 y;
 #pragma unroll
             for (int c = 0; c < 4; ++c) y[c] = gn_scaled<T>(x[u][c], f);
-            v[i + u * NVDR_GN_BLOCK] = y;
+            if (NT) __builtin_nontemporal_store(y, v + i + u * BLOCK);
+            else v[i + u * BLOCK] = y;
         }
     }
     if ((int64_t)threadIdx.x < head) one(threadIdx.x);
@@ -235,33 +268,33 @@ __device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
 }
 
 // n_part > 0: every workgroup adds the parts up itself, in the same order (a launch less than a kernel of its own for it), and the first one
-// writes the norm; n_part = 0: the factor is in out[1].
-template <int P>
-__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_scale_kernel(GradTable tab, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ out)
+// writes the norm; n_part = 0: the factor is there.  NT: the list is longer than what stays in the cache.
+template <int P, bool NT>
+__global__ void __launch_bounds__(NT ? NVDR_GN_STREAM_BLOCK : NVDR_GN_BLOCK)
+grad_scale_kernel(GradTable tab, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm, const float *__restrict__ factor)
 {
-    __shared__ double lds[NVDR_GN_BLOCK / 64];
+    __shared__ double lds[NVDR_GN_STREAM_BLOCK / 64];
     float f;
     if (n_part > 0) {
-        const double norm = gn_total<P>(part, n_part, lds);
-        f = gn_factor(norm, max_norm);
-        if (blockIdx.x == 0 && threadIdx.x == 0) {
-            out[0] = (float)norm;
-            out[1] = f;
-        }
-    } else f = out[1];
+        const double v = gn_total<P>(part, n_part, lds);
+        f = gn_factor(v, max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+    } else f = *factor;
     if (f == 1.0f) return;
-    const uint64_t chunks = tab.first[tab.n_tensors];
-    const uint32_t c0 = (uint32_t)(blockIdx.x * chunks / gridDim.x);
-    uint32_t c = (uint32_t)((blockIdx.x + 1) * chunks / gridDim.x);
-    for (int k = c > c0 ? gn_find(tab, c - 1) : 0; c > c0; --k) {
-        const uint32_t first = tab.first[k], begin = max(c0, first);
-        const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
-        char *p = (char *)(tab.data[k] & ~(3ull << 62));
-        const int64_t e0 = (int64_t)(begin - first) * len, e1 = min((int64_t)(c - first) * len, tab.n[k]);
-        if (type == GN_F32) gn_scale_part<GN_F32>(p + e0 * 4, e1 - e0, f);
-        else if (type == GN_BF16) gn_scale_part<GN_BF16>(p + e0 * 2, e1 - e0, f);
-        else gn_scale_part<GN_F16>(p + e0 * 2, e1 - e0, f);
-        c = begin;
+    const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, runs = (chunks - 1) / run + 1;
+    for (int64_t r = (int64_t)((runs - 1 - blockIdx.x) / gridDim.x) * gridDim.x + blockIdx.x; r >= 0; r -= gridDim.x) {
+        const uint32_t c0 = (uint32_t)r * run;
+        uint32_t c = min(c0 + run, chunks);
+        for (int k = gn_find(tab, c - 1); c > c0; --k) {
+            const uint32_t first = tab.first[k], begin = max(c0, first);
+            const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
+            char *p = (char *)(tab.data[k] & ~(3ull << 62));
+            const int64_t e0 = (int64_t)(begin - first) * len, e1 = min((int64_t)(c - first) * len, tab.n[k]);
+            if (type == GN_F32) gn_scale_part<GN_F32, NT>(p + e0 * 4, e1 - e0, f);
+            else if (type == GN_BF16) gn_scale_part<GN_BF16, NT>(p + e0 * 2, e1 - e0, f);
+            else gn_scale_part<GN_F16, NT>(p + e0 * 2, e1 - e0, f);
+            c = begin;
+        }
     }
 }
 
@@ -276,17 +309,17 @@ struct GradList {
 
 static int64_t gn_size(int type) { return type == GN_F32 ? 4 : 2; }
 
-static int gn_check(const GradList &l, double max_norm, const double *workspace, int64_t workspace_len, const float *out, const char *who)
+static int gn_check(const GradList &l, double max_norm, const double *workspace, int64_t workspace_len, const float *norm, const char *who)
 {
     NVDR_REQUIRE(l.count >= 0 && l.count < (1ll << 24), "%s: %lld tensors", who, (long long)l.count);
     NVDR_REQUIRE(l.count == 0 || (l.data && l.n && l.type), "%s: NULL argument", who);
-    NVDR_REQUIRE(out && workspace && ((uintptr_t)workspace & 7) == 0, "%s: out and an 8-byte aligned workspace are needed", who);
+    NVDR_REQUIRE(norm && workspace && ((uintptr_t)workspace & 7) == 0, "%s: room for the norm and an 8-byte aligned workspace are needed", who);
     NVDR_REQUIRE(workspace_len >= nvdr_grad_norm_workspace(l.count), "%s: a workspace of %lld doubles, %lld are needed", who, (long long)workspace_len,
                  (long long)nvdr_grad_norm_workspace(l.count));
     NVDR_REQUIRE(max_norm >= 0.0, "%s: max_norm has to be zero or more", who);       // (a NaN fails too)
     for (int64_t k = 0; k < l.count; ++k) {
         NVDR_REQUIRE(l.type[k] <= GN_F16, "%s: tensor %lld has type %d", who, (long long)k, (int)l.type[k]);
-        NVDR_REQUIRE(l.n[k] >= 0 && l.n[k] < (1ll << 42), "%s: tensor %lld has %lld elements", who, (long long)k, (long long)l.n[k]);
+        NVDR_REQUIRE(l.n[k] >= 0 && l.n[k] < (1ll << 40), "%s: tensor %lld has %lld elements", who, (long long)k, (long long)l.n[k]);
         NVDR_REQUIRE(l.n[k] == 0 || (l.data[k] && (uintptr_t)l.data[k] < (1ull << 62)), "%s: tensor %lld has no memory", who, (long long)k);
         NVDR_REQUIRE((uintptr_t)l.data[k] % (uintptr_t)gn_size(l.type[k]) == 0, "%s: tensor %lld is not aligned to its elements", who, (long long)k);
     }
@@ -318,8 +351,16 @@ static int gn_check_apart(const GradList &l, const char *who)
     return 0;
 }
 
-// fills `tab` with tensors from *at on, moves *at behind them; returns the workgroups of the launch (0: nothing left)
-static unsigned gn_fill(const GradList &l, int64_t *at, GradTable &tab)
+static int64_t gn_bytes(const GradList &l)
+{
+    int64_t bytes = 0;
+    for (int64_t k = 0; k < l.count; ++k) bytes += l.n[k] * gn_size(l.type[k]);
+    return bytes;
+}
+
+// fills `tab` with tensors from *at on, moves *at behind them and takes their bytes from *left; returns the workgroups of the launch, `most` at
+// most (0: nothing left)
+static unsigned gn_fill(const GradList &l, int64_t *at, int64_t *left, uint64_t most, GradTable &tab)
 {
     int m = 0;
     uint64_t chunks = 0;
@@ -329,103 +370,132 @@ static unsigned gn_fill(const GradList &l, int64_t *at, GradTable &tab)
         const int type = l.type[k];
         const uint64_t word = (uint64_t)(uintptr_t)l.data[k] | ((uint64_t)type << 62);
         const float scale = l.scale ? l.scale[k] : 1.0f;
-        const int64_t len = NVDR_GN_CHUNK / gn_size(type);
+        const int64_t size = gn_size(type), len = NVDR_GN_CHUNK / size;
         if (n == 0) { ++*at; continue; }
-        if (m && tab.data[m - 1] + (uint64_t)(tab.n[m - 1] * gn_size(type)) == word && tab.scale[m - 1] == scale) {
-            // directly behind the one before, same type and scale: one tensor
-            const uint64_t c = (uint64_t)tab.first[m - 1] + (uint64_t)((tab.n[m - 1] + n + len - 1) / len);
-            if (c >= (1ull << 31)) break;
-            tab.n[m - 1] += n;
-            chunks = c;
-        } else {
-            const uint64_t c = chunks + (uint64_t)((n + len - 1) / len);
-            if (m == NVDR_GN_TENSORS || (m && c >= (1ull << 31))) break;
+        // directly behind the one before, same type and scale: one tensor
+        const bool more = m && tab.data[m - 1] + (uint64_t)(tab.n[m - 1] * size) == word && tab.scale[m - 1] == scale;
+        const uint64_t front = more ? tab.first[m - 1] : chunks, c = front + (uint64_t)(((more ? tab.n[m - 1] : 0) + n + len - 1) / len);
+        if ((!more && m == NVDR_GN_TENSORS) || (m && c >= (1ull << 31))) break;
+        if (more) tab.n[m - 1] += n;
+        else {
             tab.data[m] = word; tab.n[m] = n; tab.scale[m] = scale;
             ++m;
-            chunks = c;
         }
+        chunks = c;
         tab.first[m] = (uint32_t)chunks;
+        *left -= n * size;
         ++*at;
     }
     tab.n_tensors = m;
-    return (unsigned)(chunks < NVDR_GN_GRID ? chunks : NVDR_GN_GRID);
+    if (chunks == 0) return 0;
+    // as few rounds as runs of NVDR_GN_RUN bytes give, all of the same length
+    const uint64_t grid = chunks < most ? chunks : most, per = NVDR_GN_RUN / NVDR_GN_CHUNK;
+    const uint64_t rounds = (chunks + grid * per - 1) / (grid * per);
+    tab.run = (uint32_t)((chunks + grid * rounds - 1) / (grid * rounds));
+    const uint64_t stay = *left >= NVDR_GN_KEEP ? 0 : (uint64_t)(NVDR_GN_KEEP - *left) / NVDR_GN_CHUNK;      // of this launch, given what follows it
+    tab.kept = (uint32_t)(stay >= chunks ? 0 : chunks - stay);
+    const uint64_t runs = (chunks + tab.run - 1) / tab.run;
+    return (unsigned)(runs < grid ? runs : grid);
 }
 
 extern "C" int64_t nvdr_grad_norm_workspace(int64_t n_tensors)
 {
     // (a launch ends with the list or with a full table; the split by the number of chunks needs more than 2^31 of them, 32 TB)
-    return ((n_tensors + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID;
+    return ((n_tensors + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID + 1;     // (the last: the factor of nvdr_grad_clip)
 }
 
+#define NVDR_GN_STARTS 64
+struct GradLaunches {
+    int64_t start[NVDR_GN_STARTS], left[NVDR_GN_STARTS];        // of the first launches: the scaling takes them in reverse
+    int64_t count = 0, end = 0;
+    int n_part = 0;
+};
+
 template <int P>
-static int gn_parts(const GradList &l, double *part, int *n_part, int *launches, hipStream_t st)
+static int gn_parts(const GradList &l, int64_t bytes, double *part, GradLaunches &g, hipStream_t st)
 {
     GradTable tab;
-    int64_t at = 0;
-    *n_part = *launches = 0;
-    while (unsigned blocks = gn_fill(l, &at, tab)) {
-        grad_norm_part_kernel<P><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part + *n_part);
+    int64_t at = 0, left = bytes;
+    for (;;) {
+        if (g.count < NVDR_GN_STARTS) { g.start[g.count] = at; g.left[g.count] = left; }
+        const unsigned blocks = gn_fill(l, &at, &left, NVDR_GN_GRID, tab);
+        if (!blocks) break;
+        grad_norm_part_kernel<P><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part + g.n_part);
         NVDR_LAUNCH_CHECK();
-        *n_part += (int)blocks;
-        ++*launches;
+        g.n_part += (int)blocks;
+        ++g.count;
     }
     return 0;
 }
 
 template <int P>
-static int gn_norm(const GradList &l, double max_norm, double *part, float *out, hipStream_t st)
+static int gn_norm(const GradList &l, double max_norm, double *part, float *norm, float *factor, hipStream_t st)
 {
-    int n_part, launches;
-    if (int r = gn_parts<P>(l, part, &n_part, &launches, st)) return r;
-    grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, n_part, max_norm, out);
+    GradLaunches g;
+    if (int r = gn_parts<P>(l, gn_bytes(l), part, g, st)) return r;
+    grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, max_norm, norm, factor);
     NVDR_LAUNCH_CHECK();
     return 0;
 }
 
 template <int P>
-static int gn_clip(const GradList &l, double max_norm, double *part, float *out, hipStream_t st)
+static int gn_clip(const GradList &l, double max_norm, double *part, float *norm, float *factor, hipStream_t st)
 {
-    int n_part, launches;
-    if (int r = gn_parts<P>(l, part, &n_part, &launches, st)) return r;
-    if (launches != 1) {
-        grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, n_part, max_norm, out);
+    GradLaunches g;
+    const int64_t bytes = gn_bytes(l);
+    if (int r = gn_parts<P>(l, bytes, part, g, st)) return r;
+    if (g.count != 1) {
+        grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, max_norm, norm, factor);
         NVDR_LAUNCH_CHECK();
-        n_part = 0;
     }
+    const int n_part = g.count == 1 ? g.n_part : 0;
+    const bool stream = bytes > NVDR_GN_KEEP;
     GradTable tab;
-    int64_t at = 0;
-    while (unsigned blocks = gn_fill(l, &at, tab)) {
-        grad_scale_kernel<P><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part, n_part, max_norm, out);
+    auto launch = [&](int64_t at, int64_t left, int64_t *behind, int64_t *after) -> bool {
+        const unsigned blocks = gn_fill(l, &at, &left, stream ? NVDR_GN_STREAM_GRID : NVDR_GN_GRID, tab);
+        if (blocks && stream) grad_scale_kernel<P, true><<<blocks, NVDR_GN_STREAM_BLOCK, 0, st>>>(tab, part, n_part, max_norm, norm, factor);
+        else if (blocks) grad_scale_kernel<P, false><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part, n_part, max_norm, norm, factor);
+        *behind = at; *after = left;
+        return blocks != 0;
+    };
+    int64_t at = 0, left = bytes;
+    const int64_t known = g.count < NVDR_GN_STARTS ? g.count : NVDR_GN_STARTS;
+    for (int64_t k = known - 1; k >= 0; --k) {
+        int64_t a, b;
+        launch(g.start[k], g.left[k], &a, &b);
         NVDR_LAUNCH_CHECK();
+        if (k == known - 1) { at = a; left = b; }
     }
+    while (known && launch(at, left, &at, &left)) NVDR_LAUNCH_CHECK();
     return 0;
 }
 
 extern "C" int nvdr_grad_norm(const void *const *data, const int64_t *n, const uint8_t *type, const float *scale, int64_t n_tensors, int norm_type, double max_norm,
-                              double *workspace, int64_t workspace_len, float *out, void *stream)
+                              double *workspace, int64_t workspace_len, float *norm, float *factor, void *stream)
 {
     NvdrRange range("nvdr_grad_norm");
     const GradList l = {data, n, type, scale, n_tensors};
-    if (int r = gn_check(l, max_norm, workspace, workspace_len, out, "nvdr_grad_norm")) return r;
+    if (int r = gn_check(l, max_norm, workspace, workspace_len, norm, "nvdr_grad_norm")) return r;
     switch (norm_type) {
-    case NVDR_NORM_INF: return gn_norm<GN_INF>(l, max_norm, workspace, out, (hipStream_t)stream);
-    case NVDR_NORM_1: return gn_norm<GN_ONE>(l, max_norm, workspace, out, (hipStream_t)stream);
-    case NVDR_NORM_2: return gn_norm<GN_TWO>(l, max_norm, workspace, out, (hipStream_t)stream);
+    case NVDR_NORM_INF: return gn_norm<GN_INF>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
+    case NVDR_NORM_1: return gn_norm<GN_ONE>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
+    case NVDR_NORM_2: return gn_norm<GN_TWO>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
     }
     NVDR_REQUIRE(false, "nvdr_grad_norm: norm type %d", norm_type);
 }
 
 extern "C" int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t *type, int64_t n_tensors, int norm_type, double max_norm, double *workspace,
-                              int64_t workspace_len, float *out, void *stream)
+                              int64_t workspace_len, float *norm, void *stream)
 {
     NvdrRange range("nvdr_grad_clip");
     const GradList l = {(const void *const *)data, n, type, nullptr, n_tensors};
-    if (int r = gn_check(l, max_norm, workspace, workspace_len, out, "nvdr_grad_clip")) return r;
+    if (int r = gn_check(l, max_norm, workspace, workspace_len, norm, "nvdr_grad_clip")) return r;
     if (int r = gn_check_apart(l, "nvdr_grad_clip")) return r;
+    float *factor = (float *)(workspace + workspace_len - 1);
     switch (norm_type) {
-    case NVDR_NORM_INF: return gn_clip<GN_INF>(l, max_norm, workspace, out, (hipStream_t)stream);
-    case NVDR_NORM_1: return gn_clip<GN_ONE>(l, max_norm, workspace, out, (hipStream_t)stream);
-    case NVDR_NORM_2: return gn_clip<GN_TWO>(l, max_norm, workspace, out, (hipStream_t)stream);
+    case NVDR_NORM_INF: return gn_clip<GN_INF>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
+    case NVDR_NORM_1: return gn_clip<GN_ONE>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
+    case NVDR_NORM_2: return gn_clip<GN_TWO>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
     }
     NVDR_REQUIRE(false, "nvdr_grad_clip: norm type %d", norm_type);
 }

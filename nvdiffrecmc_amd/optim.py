@@ -14,7 +14,6 @@ import torch
 
 from . import _lib
 
-_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # NVDR_GRAD_F32 / BF16 / F16
 _NORM_TYPES = {math.inf: 0, 1.0: 1, 2.0: 2}                                 # NVDR_NORM_INF / 1 / 2
 
 
@@ -32,53 +31,26 @@ def _max_norm(max_norm):
     return max_norm
 
 
-def _fills_its_memory(t):
-    """Whether the elements of `t` are distinct and lie without gaps, in whatever order (a permuted contiguous tensor)."""
-    need = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != need:
-            return False
-        need *= size
-    return True
+def _gradients(tensors, what, grads=False, written=False):
+    """The gradients of one call as the library takes them: (device, data, n, types, copies).  Checked there: fp32 / bf16 / fp16 on one GPU.
+    tensors: gradients, or parameters (grads: theirs are meant, None is left out).  One whose elements do not fill their memory exactly once
+    (a slice, an expanded tensor) is replaced by a contiguous copy; copies: the pairs of tensor and copy."""
+    try:
+        device, data, n, types, irregular = _lib.gradlist().collect(tensors, grads, written)
+        if not irregular:
+            return device, data, n, types, ()
+        tensors = [p.grad for p in tensors if p.grad is not None] if grads else list(tensors)
+        copies = [(tensors[i], tensors[i].detach().clone(memory_format=torch.contiguous_format)) for i in irregular]
+        for i, (_, copy) in zip(irregular, copies):
+            tensors[i] = copy
+        device, data, n, types, _ = _lib.gradlist().collect(tensors, False, False)
+        return device, data, n, types, copies
+    except (TypeError, ValueError) as e:
+        raise type(e)('%s: %s' % (what, e)) from None
 
 
-class _GradList:
-    """The tensors of one call as the lists the library takes (host memory), checked: fp32 / bf16 / fp16 on one GPU.  A tensor whose
-    elements do not lie side by side (a slice) is replaced by a contiguous copy, kept in .copies as (index, copy)."""
-
-    def __init__(self, tensors, what, scales=None):
-        try:
-            where = {t.get_device() for t in tensors}
-            self.types = bytes([_GRAD_TYPES[t.dtype] for t in tensors])
-            plain = all([t.is_contiguous() for t in tensors])
-        except (AttributeError, KeyError, TypeError):
-            for t in tensors:
-                if not isinstance(t, torch.Tensor):
-                    raise TypeError('%s: gradients must be tensors (got %s)' % (what, type(t).__name__)) from None
-                if t.dtype not in _GRAD_TYPES:
-                    raise ValueError('%s: gradients must be float32, bfloat16 or float16 (got %s)' % (what, t.dtype)) from None
-            raise
-        if len(where) > 1 or -1 in where:
-            raise RuntimeError('%s: gradients must reside on one GPU; this path has no CPU fallback' % what)
-        self.copies = []
-        if not plain:
-            tensors = list(tensors)
-            for i, t in enumerate(tensors):
-                if t.layout is not torch.strided:
-                    raise ValueError('%s: gradients must be dense (got layout %s)' % (what, t.layout))
-                if not t.is_contiguous() and not _fills_its_memory(t):
-                    tensors[i] = t.contiguous()
-                    self.copies.append((i, tensors[i]))
-        self.tensors, self.count = tensors, len(tensors)
-        self._data = array.array('Q', [t.data_ptr() for t in tensors])
-        self._n = array.array('q', [t.numel() for t in tensors])
-        self._scales = None
-        if scales is not None:
-            self._scales = array.array('f', [float(s) for s in scales])
-            if len(self._scales) != self.count:
-                raise ValueError('%s: %d scales for %d tensors' % (what, len(self._scales), self.count))
-        self.data, self.n = self._data.buffer_info()[0], self._n.buffer_info()[0]
-        self.scales = self._scales.buffer_info()[0] if self._scales is not None else None
+def _workspace(count, device):
+    return torch.empty(_lib.load().nvdr_grad_norm_workspace(count), dtype=torch.float64, device=device)
 
 
 def _on(device_index):
@@ -92,16 +64,18 @@ def grad_norm(tensors, norm_type=2.0, scales=None):
     on one GPU.  Returns a 0-d fp32 tensor on that GPU (0 on the CPU for an empty list); nothing waits for it.  Sums are kept in fp64."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
-    if not tensors:
+    if scales is not None:
+        scales = array.array('f', scales)
+        if len(scales) != len(tensors):
+            raise ValueError('grad_norm: %d scales for %d tensors' % (len(scales), len(tensors)))
+    device, data, n, types, _copies = _gradients(tensors, 'grad_norm')
+    if device < 0:
         return torch.zeros(())
-    lst = _GradList(tensors, 'grad_norm', scales)
-    lib, dev = _lib.load(), tensors[0].device
-    with _on(dev.index):
-        work = torch.empty(lib.nvdr_grad_norm_workspace(lst.count), dtype=torch.float64, device=dev)
-        out = torch.empty(2, dtype=torch.float32, device=dev)
-        _lib.check(lib.nvdr_grad_norm(lst.data, lst.n, lst.types, lst.scales, lst.count, code, math.inf, work.data_ptr(), work.numel(),
-                                      out.data_ptr(), _lib.stream_ptr()), 'grad_norm')
-    return out[0]
+    with _on(device):
+        work, norm = _workspace(len(types), device), torch.empty((), dtype=torch.float32, device=device)
+        _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0] if scales else None, len(types), code, math.inf, work.data_ptr(),
+                                              work.numel(), norm.data_ptr(), None, _lib.stream_ptr()), 'grad_norm')
+    return norm
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -112,30 +86,30 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     and raises before anything is scaled (not inside a graph capture).  max_norm = inf only measures.  Gradients must not share memory."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
-    grads = [p.grad for p in parameters if p.grad is not None]
-    if not grads:
-        return torch.zeros((), device=parameters[0].device if parameters else None)
     if error_if_nonfinite:
-        if torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError('clip_grad_norm_: error_if_nonfinite reads the norm on the host, which a graph capture does not allow')
-        norm = grad_norm(grads, norm_type)
-        if not math.isfinite(norm.item()):
-            raise RuntimeError('clip_grad_norm_: the norm of the gradients is %s' % norm.item())
-    lst = _GradList(grads, 'clip_grad_norm_')
-    for i, _ in lst.copies:
-        if any(st == 0 and sz > 1 for st, sz in zip(grads[i].stride(), grads[i].shape)):
-            raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
-    lib, dev = _lib.load(), grads[0].device
-    with _on(dev.index):
-        work = torch.empty(lib.nvdr_grad_norm_workspace(lst.count), dtype=torch.float64, device=dev)
-        out = torch.empty(2, dtype=torch.float32, device=dev)
-        _lib.check(lib.nvdr_grad_clip(lst.data, lst.n, lst.types, lst.count, code, max_norm, work.data_ptr(), work.numel(),
-                                      out.data_ptr(), _lib.stream_ptr()), 'clip_grad_norm_')
-        with torch.no_grad():
-            for i, copy in lst.copies:
-                grads[i].copy_(copy)
-    torch.autograd.graph.increment_version(grads)
-    return out[0]
+        norm = grad_norm([p.grad for p in parameters if p.grad is not None], norm_type).item()
+        if not math.isfinite(norm):
+            raise RuntimeError('clip_grad_norm_: the norm of the gradients is %s' % norm)
+    device, data, n, types, copies = _gradients(parameters, 'clip_grad_norm_', grads=True, written=True)
+    if device < 0:
+        return torch.zeros((), device=parameters[0].device if parameters else None)
+    for g, _ in copies:
+        reach = 0
+        for stride, size in sorted((st, sz) for st, sz in zip(g.stride(), g.shape) if sz != 1):
+            if stride <= reach:
+                raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
+            reach += (size - 1) * stride
+    with _on(device):
+        work, norm = _workspace(len(types), device), torch.empty((), dtype=torch.float32, device=device)
+        _lib.check(_lib.load().nvdr_grad_clip(data, n, types, len(types), code, max_norm, work.data_ptr(), work.numel(), norm.data_ptr(),
+                                              _lib.stream_ptr()), 'clip_grad_norm_')
+        if copies:
+            with torch.no_grad():
+                for g, copy in copies:
+                    g.copy_(copy)
+    return norm
 
 
 class FusedAdam:
@@ -174,7 +148,8 @@ class FusedAdam:
         self._measured = False
         dev = self.params[0].device
         self._norm_out = torch.zeros(2, dtype=torch.float32, device=dev) if max_norm is not None else None       # norm, factor
-        self._norm_work = torch.empty(_lib.load().nvdr_grad_norm_workspace(len(self.params)), dtype=torch.float64, device=dev) if max_norm is not None else None
+        self._norm_view = self._norm_out[0] if max_norm is not None else None
+        self._norm_work = _workspace(len(self.params), dev) if max_norm is not None else None
         self.state = torch.zeros(8, dtype=torch.int32, device=self.params[0].device)     # steps taken, scratch, beta1^t, beta2^t (doubles)
 
     @property
@@ -184,7 +159,7 @@ class FusedAdam:
     @property
     def grad_norm(self):
         """Norm of the gradients of the last step before clipping (0 before the first one; None without max_norm)."""
-        return None if self._norm_out is None else self._norm_out[0]
+        return self._norm_view
 
     def measure_norm(self, grad_mult=1.0):
         """The norm of this iteration's gradients into .grad_norm, and the factor of the updates that follow (max_norm).  step() calls it;
@@ -195,11 +170,11 @@ class FusedAdam:
         for i in live:
             if self.params[i].grad is None:
                 raise RuntimeError('FusedAdam.step: parameter %d has no gradient' % i)
-        lst = _GradList([self.params[i].grad for i in live], 'FusedAdam', [float(self.grad_scales[i]) * float(grad_mult) for i in live])
-        lib, dev = _lib.load(), self.params[0].device
-        with _on(dev.index):
-            _lib.check(lib.nvdr_grad_norm(lst.data, lst.n, lst.types, lst.scales, lst.count, self._norm_code, self.max_norm, self._norm_work.data_ptr(),
-                                          self._norm_work.numel(), self._norm_out.data_ptr(), _lib.stream_ptr()), 'grad_norm')
+        scales = array.array('f', [float(self.grad_scales[i]) * float(grad_mult) for i in live])
+        device, data, n, types, _copies = _gradients([self.params[i].grad for i in live], 'FusedAdam')
+        with _on(self.state.get_device()):
+            _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0], len(types), self._norm_code, self.max_norm, self._norm_work.data_ptr(),
+                                                  self._norm_work.numel(), self._norm_out.data_ptr(), self._norm_out.data_ptr() + 4, _lib.stream_ptr()), 'grad_norm')
         self._measured = True
 
     def zero_grad(self, set_to_none=True):

@@ -313,6 +313,66 @@ def test_more_elements_than_32_bits_count(dev):
     close(lo, 2.0 ** -10 * f, 2.0 ** -8 + 2.0 ** -23)
 
 
+@pytest.mark.parametrize('p', [2.0, 1.0, math.inf], ids=['two', 'one', 'max'])
+def test_lists_longer_than_the_cache(p, dev):
+    """Over 160 MB: streamed in several rounds of runs, the end kept in the cache, scaled from the end by larger workgroups.  Three tables,
+    odd lengths, odd places, all types; the reference sums in fp64 on the GPU."""
+    from nvdiffrecmc_amd.optim import clip_grad_norm_, grad_norm
+    gen = torch.Generator(device=dev).manual_seed(3)
+    spec = [(30000001, F32), (7, F16), (50000003, BF16)] + [(1 + 13 * k, (F32, BF16, F16)[k % 3]) for k in range(400)] + [(20000005, F16), (3000001, F32)]
+    grads, kept = [], []
+    for k, (n, t) in enumerate(spec):
+        b = torch.empty(n + 5, dtype=t, device=dev)
+        b.normal_(generator=gen)
+        grads.append(b[k % 4:k % 4 + n])
+        kept.append((b, b.clone()))
+    before = [g.clone() for g in grads]
+    big = lambda g: g.double().abs()
+    if p == math.inf:
+        want = max(float(big(g).max()) for g in grads)
+    else:
+        want = sum(float((big(g) ** p).sum()) for g in grads) ** (1.0 / p)
+    n = grad_norm(grads, norm_type=p)
+    close(float(n), want, NORM_TOL)
+    m = clip_grad_norm_(params_of(grads), 0.37 * want, norm_type=p)
+    assert m.item() == n.item()
+    f = factor64(want, 0.37 * want)
+    for k, (g, b, (buf, old)) in enumerate(zip(grads, before, kept)):
+        tol = (2.0 ** -23 + HALF_STEP[g.dtype]) * big(b) * f + SUBNORMAL[g.dtype] / 2 + 2.0 ** -150
+        assert not bool(((g.double() - b.double() * f).abs() > tol).any()), k
+        assert torch.equal(buf[:k % 4], old[:k % 4]) and torch.equal(buf[k % 4 + g.numel():], old[k % 4 + g.numel():]), k
+
+
+def test_more_launches_than_the_reverse_order_remembers(dev):
+    """65 tables and more: the ones behind the 64th are scaled in their own order, each tensor once."""
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    count = 160 * 66 + 7
+    buf = values(count * 4, 11, F32)                                       # every fourth element: no two are neighbours
+    d = buf.to(dev)
+    grads = list(d.view(count, 4)[:, :1].unbind(0))
+    h = buf.view(count, 4)[:, 0]
+    want = norm64([h], 2.0)
+    n = clip_grad_norm_(params_of(grads), 0.5 * want)
+    close(n.item(), want, NORM_TOL)
+    assert_scaled(d.view(count, 4)[:, 0], h, factor64(want, 0.5 * want))
+    assert torch.equal(d.view(count, 4)[:, 1:].cpu(), buf.view(count, 4)[:, 1:])
+
+
+def test_columns_of_one_buffer(dev):
+    """Gradients that interleave in memory: each is scaled through its own copy, once."""
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    h = values(60 * 70, 12, F32).view(60, 70)
+    d = h.to(dev)
+    want = norm64([h], 2.0)
+    n = clip_grad_norm_(params_of([d[:, :11], d[:, 11:40], d[:, 40:]]), 0.5 * want)
+    close(n.item(), want, NORM_TOL)
+    assert_scaled(d, h, factor64(want, 0.5 * want))
+    p = torch.nn.Parameter(torch.empty(10, 8, device=dev))
+    p.grad = d.view(-1).as_strided((10, 8), (5, 1))                        # rows that overlap
+    with pytest.raises(RuntimeError, match='share memory'):
+        clip_grad_norm_(p, 1e-3)
+
+
 # ---- the clipped step ------------------------------------------------------------------------------------------------------------------
 
 def _adam(shapes, dev, seed, **kw):

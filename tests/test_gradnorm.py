@@ -25,8 +25,10 @@ def test_python_refusals():
         for p in (0.0, 3.0, -math.inf, math.nan):
             with pytest.raises(ValueError, match='norm_type'):
                 call(x, norm_type=p)
-    with pytest.raises(TypeError, match='float'):
+    with pytest.raises(TypeError, match='grad_norm.*float'):
         optim.grad_norm([1.0])
+    with pytest.raises(TypeError, match='clip_grad_norm_.*str'):
+        optim.clip_grad_norm_(['w'], 1.0)
     with pytest.raises(RuntimeError):
         optim.grad_norm([torch.eye(3).to_sparse()])
     for m in (-1.0, math.nan, -math.inf):
@@ -42,24 +44,17 @@ def test_nothing_to_do():
     assert optim.clip_grad_norm_((p for p in ()), 1.0).item() == 0.0
 
 
-def test_permuted_and_sliced_layouts_are_told_apart():
-    x = torch.zeros(4, 5, 6)
-    for t, want in ((x, True), (x.permute(2, 0, 1), True), (x.transpose(0, 2), True), (x[:, :, :3], False), (x[::2], False), (x[:1], True),
-                    (torch.zeros(1).expand(7), False), (x.permute(1, 0, 2)[:2], False), (x[:, :1].transpose(0, 1), False), (torch.zeros(()), True)):
-        assert optim._fills_its_memory(t) == want, (t.shape, t.stride())
-
-
 # ---- the C entries refuse before anything is launched -----------------------------------------------------------------------------------
 
 def _call(entry, data, n, types, max_norm=1.0, norm_type=2, workspace=None, out=True, scale=None):
     """The entry on host lists (addresses are never dereferenced: every call here is refused)."""
     lib = _lib.load()
-    d, c = array.array('Q', data), array.array('q', n)
+    d, c = array.array('Q', data).tobytes(), array.array('q', n).tobytes()
     need = lib.nvdr_grad_norm_workspace(len(n))
     ws = torch.empty(need if workspace is None else workspace, dtype=torch.float64)
     o = torch.empty(2)
-    args = [d.buffer_info()[0], c.buffer_info()[0], bytes(types)] + ([scale] if entry == 'nvdr_grad_norm' else [])
-    args += [len(n), norm_type, max_norm, ws.data_ptr(), ws.numel(), o.data_ptr() if out else None, None]
+    args = [d, c, bytes(types)] + ([scale] if entry == 'nvdr_grad_norm' else [])
+    args += [len(n), norm_type, max_norm, ws.data_ptr(), ws.numel(), o.data_ptr() if out else None] + ([None] if entry == 'nvdr_grad_norm' else []) + [None]
     rc = getattr(lib, entry)(*args)
     return rc, (lib.nvdr_last_error() or b'').decode()
 
@@ -70,12 +65,12 @@ def test_entries_refuse_bad_arguments(entry):
     cases = [
         (dict(data=[A], n=[4], types=[3]), 'type'),
         (dict(data=[A], n=[-1], types=[0]), 'elements'),
-        (dict(data=[A], n=[1 << 42], types=[0]), 'elements'),
+        (dict(data=[A], n=[1 << 40], types=[0]), 'elements'),
         (dict(data=[0], n=[4], types=[0]), 'no memory'),
         (dict(data=[A + 2], n=[4], types=[0]), 'aligned'),
         (dict(data=[A + 1], n=[4], types=[1]), 'aligned'),
         (dict(data=[A], n=[4], types=[0], workspace=8), 'workspace'),
-        (dict(data=[A], n=[4], types=[0], out=False), 'out'),
+        (dict(data=[A], n=[4], types=[0], out=False), 'norm'),
         (dict(data=[A], n=[4], types=[0], max_norm=-1.0), 'max_norm'),
         (dict(data=[A], n=[4], types=[0], max_norm=math.nan), 'max_norm'),
         (dict(data=[A], n=[4], types=[0], norm_type=3), 'norm type'),
@@ -86,7 +81,7 @@ def test_entries_refuse_bad_arguments(entry):
         assert rc == -1 and word in msg, (kw, rc, msg)
     lib = _lib.load()
     ws, o = torch.empty(8192, dtype=torch.float64), torch.empty(2)
-    tail = [2, 1.0, ws.data_ptr(), ws.numel(), o.data_ptr(), None]
+    tail = [2, 1.0, ws.data_ptr(), ws.numel(), o.data_ptr()] + ([None] if entry == 'nvdr_grad_norm' else []) + [None]
     assert getattr(lib, entry)(*([None, None, None] + ([None] if entry == 'nvdr_grad_norm' else []) + [1] + tail)) == -1
     assert getattr(lib, entry)(*([None, None, None] + ([None] if entry == 'nvdr_grad_norm' else []) + [-1] + tail)) == -1
 
@@ -102,6 +97,14 @@ def test_workspace_grows_with_the_list():
     lib = _lib.load()
     sizes = [lib.nvdr_grad_norm_workspace(n) for n in (0, 1, 160, 161, 1000)]
     assert sizes[0] > 0 and sizes == sorted(sizes) and sizes[1] == sizes[2] < sizes[3] < sizes[4]
+
+
+def test_a_missing_extension_is_an_error(monkeypatch):
+    from nvdiffrecmc_amd import _build
+    monkeypatch.setattr(_lib, '_gradlist', None)
+    monkeypatch.setattr(_build, 'GRADLIST', '/nonexistent/_gradlist.so')
+    with pytest.raises(RuntimeError, match='not built'):
+        optim.grad_norm([torch.zeros(3)])
 
 
 def test_adam_entry_refuses_without_a_launch():

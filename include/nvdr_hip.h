@@ -489,21 +489,26 @@ int nvdr_adam_step_partial(const nvdr_adam_tensor *tensors, int n_tensors, doubl
 
 /* The same update with every gradient also multiplied by *grad_factor (device memory, read by the launch; NULL: one): the factor of
  * nvdr_grad_norm, so that clipping takes no pass of its own over the gradients.  The gradients themselves stay as they are. */
+int nvdr_adam_step_factor(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps, int *state,
+                          int advance, const float *grad_factor, void *stream);
+/* A whole step with clipping: the norm (norm_type, see nvdr_grad_norm) of grad * grad_scale over the tensors that are not frozen into *norm, then
+ * the update of all of them with factor = min(1, max_norm / (norm + 1e-6)).  The kernel that finishes the norm moves the step counter.
+ * workspace: 16-byte aligned, 2 + nvdr_grad_norm_workspace(..., 0) doubles for these tensors. */
 int nvdr_adam_step_clipped(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps, int *state,
-                           int advance, const float *grad_factor, void *stream);
+                           int norm_type, double max_norm, double *workspace, int64_t workspace_len, float *norm, void *stream);
 
 /* ---- the global norm of many gradient tensors, and clipping by it (additive; the reference does not clip).
  *     norm   = (sum_k sum_i |scale[k] data[k][i]|^p)^(1/p), p = 1 or 2; the largest magnitude for NVDR_NORM_INF (a NaN anywhere gives a NaN)
  *     factor = min(1, max_norm / (norm + 1e-6)); one for an infinite max_norm
  * data[k]: n[k] contiguous elements of type[k] in any mixture, aligned to their own size; n[k] = 0 is skipped.  scale: NULL for ones.  The
  * four lists live in HOST memory and are read before the call returns (a captured graph keeps them).  Sums in fp64, in an order that depends
- * on sizes and alignment only.  workspace: nvdr_grad_norm_workspace(n_tensors) doubles of device memory, nothing to initialise; launches that
- * may run at the same time need one each.  norm, factor: one float each in device memory (factor may be NULL).
+ * on sizes and alignment only.  workspace: nvdr_grad_norm_workspace(n, type, n_tensors, clip) doubles of device memory (none for a short list,
+ * which one workgroup takes), 8-byte aligned, nothing to initialise; launches that may run at the same time need one each.  norm, factor: one float each in device memory (factor may be NULL).
  * nvdr_grad_norm leaves the gradients alone; nvdr_grad_clip multiplies them by the factor in place (computed in fp32, one rounding to the
  * element's type) and writes nothing when the factor is one.  Gradients of nvdr_grad_clip must not share memory. */
 enum { NVDR_GRAD_F32 = 0, NVDR_GRAD_BF16 = 1, NVDR_GRAD_F16 = 2 };
 enum { NVDR_NORM_INF = 0, NVDR_NORM_1 = 1, NVDR_NORM_2 = 2 };
-int64_t nvdr_grad_norm_workspace(int64_t n_tensors);
+int64_t nvdr_grad_norm_workspace(const int64_t *n, const uint8_t *type, int64_t n_tensors, int clip);
 int nvdr_grad_norm(const void *const *data, const int64_t *n, const uint8_t *type, const float *scale, int64_t n_tensors, int norm_type,
                    double max_norm, double *workspace, int64_t workspace_len, float *norm, float *factor, void *stream);
 int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t *type, int64_t n_tensors, int norm_type, double max_norm,

@@ -173,8 +173,9 @@ _SIGNATURES = {
     'nvdr_light_update_pdf': [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],
     'nvdr_adam_step': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_void_p],
     'nvdr_adam_step_partial': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p],
-    'nvdr_adam_step_clipped': [ctypes.POINTER(NvdrAdamTensor), c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p, c_void_p],
-    'nvdr_grad_norm_workspace': [c_int64],
+    'nvdr_adam_step_factor': [ctypes.c_char_p, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, c_void_p, c_void_p],
+    'nvdr_adam_step_clipped': [ctypes.c_char_p, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_void_p, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
+    'nvdr_grad_norm_workspace': [ctypes.c_char_p, ctypes.c_char_p, c_int64, c_int],
     'nvdr_grad_norm': [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, c_void_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
     'nvdr_grad_clip': [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, c_int64, c_int, ctypes.c_double, c_void_p, c_int64, c_void_p, c_void_p],
     'nvdr_abi_sizeof': [c_int],
@@ -254,7 +255,8 @@ def check(rc, what):
 
 
 def stream_ptr():
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the handle alone: building a torch.cuda.Stream object for it costs 2.8 us a call)
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def ptr(t):

@@ -33,6 +33,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "gradnorm.h"
 #include "nvdr_hip.h"
 
 #define NVDR_GN_BLOCK 512               // threads of a workgroup of the norm, and of the scaling of a list that fits the cache
@@ -43,6 +44,10 @@
 #define NVDR_GN_CHUNK 4096              // bytes
 #define NVDR_GN_RUN (128 << 10)         // bytes
 #define NVDR_GN_KEEP (160ll << 20)      // bytes that stay in the last-level cache (256 MB) from one pass to the next: 96 to 256 MB within 2 %
+#define NVDR_GN_ONE_BLOCK 1024          // a short list: one workgroup does all of it
+#define NVDR_GN_ONE_TENSORS 8
+#define NVDR_GN_ONE_NORM (256 << 10)    // bytes
+#define NVDR_GN_ONE_CLIP (64 << 10)     // bytes
 #define NVDR_GN_EPS 1e-6
 
 enum { GN_INF = 0, GN_ONE = 1, GN_TWO = 2 };                // the kernels' norm types
@@ -127,7 +132,7 @@ __device__ __forceinline__ int gn_chunk_len(int type) { return type == GN_F32 ? 
 template <bool NT>
 __device__ __forceinline__ gn_u4 gn_load(const gn_u4 *p) { return NT ? __builtin_nontemporal_load(p) : *p; }
 
-template <int P, int T, bool NT>
+template <int P, int T, bool NT, int BLOCK>
 __device__ __forceinline__ double gn_sum_part(const char *p, int64_t count)
 {
     constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE;
@@ -143,33 +148,33 @@ __device__ __forceinline__ double gn_sum_part(const char *p, int64_t count)
     if ((int64_t)threadIdx.x < tail) a[1].add(one(head + nvec * VEC + threadIdx.x));
     const gn_u4 *v = (const gn_u4 *)(p + head * SIZE);
     int64_t i = threadIdx.x;
-    for (; i + 3 * NVDR_GN_BLOCK < nvec; i += 4 * NVDR_GN_BLOCK) {      // four loads in flight
+    for (; i + 3 * BLOCK < nvec; i += 4 * BLOCK) {      // four loads in flight
         gn_u4 x[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = gn_load<NT>(v + i + u * NVDR_GN_BLOCK);
+        for (int u = 0; u < 4; ++u) x[u] = gn_load<NT>(v + i + u * BLOCK);
 #pragma unroll
         for (int u = 0; u < 4; ++u) a[u].template add16<T>(x[u]);
     }
     gn_u4 x[3];
 #pragma unroll
-    for (int u = 0; u < 3; ++u) x[u] = i + u * NVDR_GN_BLOCK < nvec ? gn_load<NT>(v + i + u * NVDR_GN_BLOCK) : gn_u4{0, 0, 0, 0};     // (a zero adds nothing)
+    for (int u = 0; u < 3; ++u) x[u] = i + u * BLOCK < nvec ? gn_load<NT>(v + i + u * BLOCK) : gn_u4{0, 0, 0, 0};     // (a zero adds nothing)
 #pragma unroll
     for (int u = 0; u < 3; ++u) a[u].template add16<T>(x[u]);
     return gn_join<P>(gn_join<P>(a[0].value(), a[1].value()), gn_join<P>(a[2].value(), a[3].value()));
 }
 
-template <int P, bool NT>
+template <int P, bool NT, int BLOCK>
 __device__ __forceinline__ double gn_sum_typed(const char *p, int type, int64_t e0, int64_t e1)
 {
-    if (type == GN_F32) return gn_sum_part<P, GN_F32, NT>(p + e0 * 4, e1 - e0);
-    if (type == GN_BF16) return gn_sum_part<P, GN_BF16, NT>(p + e0 * 2, e1 - e0);
-    return gn_sum_part<P, GN_F16, NT>(p + e0 * 2, e1 - e0);
+    if (type == GN_F32) return gn_sum_part<P, GN_F32, NT, BLOCK>(p + e0 * 4, e1 - e0);
+    if (type == GN_BF16) return gn_sum_part<P, GN_BF16, NT, BLOCK>(p + e0 * 2, e1 - e0);
+    return gn_sum_part<P, GN_F16, NT, BLOCK>(p + e0 * 2, e1 - e0);
 }
 
-template <int P>
-__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_part_kernel(GradTable tab, double *__restrict__ part)
+// one thread's sum over the runs of its workgroup
+template <int P, int BLOCK>
+__device__ __forceinline__ double gn_sum_runs(const GradTable &tab)
 {
-    __shared__ double lds[NVDR_GN_BLOCK / 64];
     const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, kept = tab.kept;
     double sum = 0.0;
     for (uint64_t r = (uint64_t)blockIdx.x * run; r < chunks; r += (uint64_t)gridDim.x * run) {
@@ -182,25 +187,34 @@ __global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_part_kernel(GradTable
             const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
             const char *p = (const char *)(tab.data[k] & ~(3ull << 62));
             const int64_t e0 = (int64_t)(c - first) * len, e1 = min((int64_t)(end - first) * len, tab.n[k]);
-            const double s = stream ? gn_sum_typed<P, true>(p, type, e0, e1) : gn_sum_typed<P, false>(p, type, e0, e1);
+            const double s = stream ? gn_sum_typed<P, true, BLOCK>(p, type, e0, e1) : gn_sum_typed<P, false, BLOCK>(p, type, e0, e1);
             const double w = fabs((double)tab.scale[k]);
             sum = gn_join<P>(sum, P == GN_TWO ? s * (w * w) : s * w);
             c = end;
             k += end == next;
         }
     }
-    sum = gn_block_join<P>(sum, lds);
+    return sum;
+}
+
+template <int P>
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_part_kernel(GradTable tab, double *__restrict__ part)
+{
+    __shared__ double lds[NVDR_GN_BLOCK / 64];
+    const double sum = gn_block_join<P>(gn_sum_runs<P, NVDR_GN_BLOCK>(tab), lds);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
 
 // ---- the norm of the parts, and the factor -----------------------------------------------------------------------------------------
 template <int P>
+__device__ __forceinline__ double gn_root(double v) { return P == GN_TWO ? sqrt(v) : v; }
+
+template <int P>
 __device__ __forceinline__ double gn_total(const double *__restrict__ part, int n_part, double *lds)
 {
     double v = 0.0;
     for (int i = threadIdx.x; i < n_part; i += blockDim.x) v = gn_join<P>(v, part[i]);
-    v = gn_block_join<P>(v, lds);
-    return P == GN_TWO ? sqrt(v) : v;
+    return gn_root<P>(gn_block_join<P>(v, lds));
 }
 
 // one rounding to fp32, of the quotient in fp64; a NaN stays a NaN.  An infinite max_norm never scales (inf / inf would)
@@ -211,15 +225,42 @@ __device__ __forceinline__ float gn_factor(double norm, double max_norm)
     return (float)(f > 1.0 ? 1.0 : f);
 }
 
+struct GradOut {
+    double max_norm;
+    float *norm, *factor;       // factor: NULL for none
+    AdamBegin adam;             // adam.state: NULL for none
+};
+
+// what one thread writes when the norm is known.  In front of an Adam step also what that needs of its counter, which moves here: the
+// update reads no state, and no launch behind it is needed to move it
+__device__ __forceinline__ void gn_finish(double norm, const GradOut &o)
+{
+    const float f = gn_factor(norm, o.max_norm);
+    *o.norm = (float)norm;
+    if (o.factor) *o.factor = f;
+    if (o.adam.state) {
+        AdamStep s = adam_begin(o.adam.state, o.adam.lr, o.adam.beta1, o.adam.beta2);
+        s.factor = f;
+        *o.adam.step = s;
+        adam_advance(o.adam.state, o.adam.beta1, o.adam.beta2);
+    }
+}
+
 template <int P>
-__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_final_kernel(const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm, float *__restrict__ factor)
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_final_kernel(const double *__restrict__ part, int n_part, GradOut out)
 {
     __shared__ double lds[NVDR_GN_BLOCK / 64];
-    const double v = gn_total<P>(part, n_part, lds);
-    if (threadIdx.x == 0) {
-        *norm = (float)v;
-        if (factor) *factor = gn_factor(v, max_norm);
-    }
+    const double norm = gn_total<P>(part, n_part, lds);
+    if (threadIdx.x == 0) gn_finish(norm, out);
+}
+
+// a short list: all of it by one workgroup, in one launch and without parts
+template <int P>
+__global__ void __launch_bounds__(NVDR_GN_ONE_BLOCK) grad_norm_one_kernel(GradTable tab, GradOut out)
+{
+    __shared__ double lds[NVDR_GN_ONE_BLOCK / 64];
+    const double norm = gn_root<P>(gn_block_join<P>(gn_sum_runs<P, NVDR_GN_ONE_BLOCK>(tab), lds));
+    if (threadIdx.x == 0) gn_finish(norm, out);
 }
 
 // ---- scaling -------------------------------------------------------------------------------------------------------------------------
@@ -236,10 +277,10 @@ __device__ __forceinline__ uint32_t gn_scaled(uint32_t w, float f)
 }
 
 // from the end to the front: the norm's pass went the other way, and what it read last is still in the last-level cache
-template <int T, bool NT>
+template <int T, bool NT, int BLOCK>
 __device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
 {
-    constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE, BLOCK = NT ? NVDR_GN_STREAM_BLOCK : NVDR_GN_BLOCK, DEEP = NT ? 8 : 4;
+    constexpr int SIZE = T == GN_F32 ? 4 : 2, VEC = 16 / SIZE, DEEP = NT ? 8 : 4;
     auto one = [&](int64_t i) {
         if (T == GN_F32) ((float *)p)[i] *= f;
         else ((uint16_t *)p)[i] = (uint16_t)gn_scaled<T>(((uint16_t *)p)[i], f);
@@ -267,6 +308,26 @@ __device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
     if ((int64_t)threadIdx.x < tail) one(head + nvec * VEC + threadIdx.x);
 }
 
+template <bool NT, int BLOCK>
+__device__ __forceinline__ void gn_scale_runs(const GradTable &tab, float f)
+{
+    const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, runs = (chunks - 1) / run + 1;
+    for (int64_t r = (int64_t)((runs - 1 - blockIdx.x) / gridDim.x) * gridDim.x + blockIdx.x; r >= 0; r -= gridDim.x) {
+        const uint32_t c0 = (uint32_t)r * run;
+        uint32_t c = min(c0 + run, chunks);
+        for (int k = gn_find(tab, c - 1); c > c0; --k) {
+            const uint32_t first = tab.first[k], begin = max(c0, first);
+            const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
+            char *p = (char *)(tab.data[k] & ~(3ull << 62));
+            const int64_t e0 = (int64_t)(begin - first) * len, e1 = min((int64_t)(c - first) * len, tab.n[k]);
+            if (type == GN_F32) gn_scale_part<GN_F32, NT, BLOCK>(p + e0 * 4, e1 - e0, f);
+            else if (type == GN_BF16) gn_scale_part<GN_BF16, NT, BLOCK>(p + e0 * 2, e1 - e0, f);
+            else gn_scale_part<GN_F16, NT, BLOCK>(p + e0 * 2, e1 - e0, f);
+            c = begin;
+        }
+    }
+}
+
 // n_part > 0: every workgroup adds the parts up itself, in the same order (a launch less than a kernel of its own for it), and the first one
 // writes the norm; n_part = 0: the factor is there.  NT: the list is longer than what stays in the cache.
 template <int P, bool NT>
@@ -281,21 +342,18 @@ grad_scale_kernel(GradTable tab, const double *__restrict__ part, int n_part, do
         if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
     } else f = *factor;
     if (f == 1.0f) return;
-    const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, runs = (chunks - 1) / run + 1;
-    for (int64_t r = (int64_t)((runs - 1 - blockIdx.x) / gridDim.x) * gridDim.x + blockIdx.x; r >= 0; r -= gridDim.x) {
-        const uint32_t c0 = (uint32_t)r * run;
-        uint32_t c = min(c0 + run, chunks);
-        for (int k = gn_find(tab, c - 1); c > c0; --k) {
-            const uint32_t first = tab.first[k], begin = max(c0, first);
-            const int type = (int)(tab.data[k] >> 62), len = gn_chunk_len(type);
-            char *p = (char *)(tab.data[k] & ~(3ull << 62));
-            const int64_t e0 = (int64_t)(begin - first) * len, e1 = min((int64_t)(c - first) * len, tab.n[k]);
-            if (type == GN_F32) gn_scale_part<GN_F32, NT>(p + e0 * 4, e1 - e0, f);
-            else if (type == GN_BF16) gn_scale_part<GN_BF16, NT>(p + e0 * 2, e1 - e0, f);
-            else gn_scale_part<GN_F16, NT>(p + e0 * 2, e1 - e0, f);
-            c = begin;
-        }
-    }
+    gn_scale_runs<NT, NT ? NVDR_GN_STREAM_BLOCK : NVDR_GN_BLOCK>(tab, f);
+}
+
+// a short list: the norm and the scaling by one workgroup.  The barriers of the sum lie between the last read and the first write.
+template <int P>
+__global__ void __launch_bounds__(NVDR_GN_ONE_BLOCK) grad_clip_one_kernel(GradTable tab, double max_norm, float *__restrict__ norm)
+{
+    __shared__ double lds[NVDR_GN_ONE_BLOCK / 64];
+    const double v = gn_root<P>(gn_block_join<P>(gn_sum_runs<P, NVDR_GN_ONE_BLOCK>(tab), lds));
+    if (threadIdx.x == 0) *norm = (float)v;
+    const float f = gn_factor(v, max_norm);
+    if (f != 1.0f && tab.n_tensors) gn_scale_runs<false, NVDR_GN_ONE_BLOCK>(tab, f);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
@@ -309,13 +367,28 @@ struct GradList {
 
 static int64_t gn_size(int type) { return type == GN_F32 ? 4 : 2; }
 
-static int gn_check(const GradList &l, double max_norm, const double *workspace, int64_t workspace_len, const float *norm, const char *who)
+static int64_t gn_bytes(const GradList &l)
+{
+    int64_t bytes = 0;
+    for (int64_t k = 0; k < l.count; ++k) bytes += l.n[k] * gn_size(l.type[k]);
+    return bytes;
+}
+
+static bool gn_one(const GradList &l, int64_t bytes, int64_t most) { return l.count <= NVDR_GN_ONE_TENSORS && bytes <= most; }
+
+static int64_t gn_workspace(const GradList &l, int64_t bytes, int64_t most)
+{
+    if (gn_one(l, bytes, most)) return 0;
+    // (a launch ends with the list or with a full table; the split by the number of chunks needs more than 2^31 of them, 8 TB)
+    return ((l.count + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID + 1;      // (the last: the factor of nvdr_grad_clip)
+}
+
+static int gn_check(const GradList &l, int norm_type, double max_norm, int64_t most, const double *workspace, int64_t workspace_len, const float *norm, const char *who)
 {
     NVDR_REQUIRE(l.count >= 0 && l.count < (1ll << 24), "%s: %lld tensors", who, (long long)l.count);
     NVDR_REQUIRE(l.count == 0 || (l.data && l.n && l.type), "%s: NULL argument", who);
-    NVDR_REQUIRE(norm && workspace && ((uintptr_t)workspace & 7) == 0, "%s: room for the norm and an 8-byte aligned workspace are needed", who);
-    NVDR_REQUIRE(workspace_len >= nvdr_grad_norm_workspace(l.count), "%s: a workspace of %lld doubles, %lld are needed", who, (long long)workspace_len,
-                 (long long)nvdr_grad_norm_workspace(l.count));
+    NVDR_REQUIRE(norm, "%s: room for the norm is needed", who);
+    NVDR_REQUIRE(norm_type == NVDR_NORM_INF || norm_type == NVDR_NORM_1 || norm_type == NVDR_NORM_2, "%s: norm type %d", who, norm_type);
     NVDR_REQUIRE(max_norm >= 0.0, "%s: max_norm has to be zero or more", who);       // (a NaN fails too)
     for (int64_t k = 0; k < l.count; ++k) {
         NVDR_REQUIRE(l.type[k] <= GN_F16, "%s: tensor %lld has type %d", who, (long long)k, (int)l.type[k]);
@@ -323,6 +396,9 @@ static int gn_check(const GradList &l, double max_norm, const double *workspace,
         NVDR_REQUIRE(l.n[k] == 0 || (l.data[k] && (uintptr_t)l.data[k] < (1ull << 62)), "%s: tensor %lld has no memory", who, (long long)k);
         NVDR_REQUIRE((uintptr_t)l.data[k] % (uintptr_t)gn_size(l.type[k]) == 0, "%s: tensor %lld is not aligned to its elements", who, (long long)k);
     }
+    const int64_t need = gn_workspace(l, gn_bytes(l), most);
+    NVDR_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 7) == 0 && workspace_len >= need), "%s: an 8-byte aligned workspace of %lld doubles is needed, there are %lld",
+                 who, (long long)need, (long long)(workspace ? workspace_len : 0));
     return 0;
 }
 
@@ -349,13 +425,6 @@ static int gn_check_apart(const GradList &l, const char *who)
     free(s);
     NVDR_REQUIRE(apart, "%s: two gradients share memory (the same tensor twice, or overlapping views)", who);
     return 0;
-}
-
-static int64_t gn_bytes(const GradList &l)
-{
-    int64_t bytes = 0;
-    for (int64_t k = 0; k < l.count; ++k) bytes += l.n[k] * gn_size(l.type[k]);
-    return bytes;
 }
 
 // fills `tab` with tensors from *at on, moves *at behind them and takes their bytes from *left; returns the workgroups of the launch, `most` at
@@ -387,6 +456,8 @@ static unsigned gn_fill(const GradList &l, int64_t *at, int64_t *left, uint64_t 
         ++*at;
     }
     tab.n_tensors = m;
+    tab.run = 1;
+    tab.kept = 0;
     if (chunks == 0) return 0;
     // as few rounds as runs of NVDR_GN_RUN bytes give, all of the same length
     const uint64_t grid = chunks < most ? chunks : most, per = NVDR_GN_RUN / NVDR_GN_CHUNK;
@@ -398,10 +469,11 @@ static unsigned gn_fill(const GradList &l, int64_t *at, int64_t *left, uint64_t 
     return (unsigned)(runs < grid ? runs : grid);
 }
 
-extern "C" int64_t nvdr_grad_norm_workspace(int64_t n_tensors)
+extern "C" int64_t nvdr_grad_norm_workspace(const int64_t *n, const uint8_t *type, int64_t n_tensors, int clip)
 {
-    // (a launch ends with the list or with a full table; the split by the number of chunks needs more than 2^31 of them, 32 TB)
-    return ((n_tensors + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID + 1;     // (the last: the factor of nvdr_grad_clip)
+    const GradList l = {nullptr, n, type, nullptr, n_tensors};
+    if (n_tensors < 0 || (n_tensors && (!n || !type))) return 0;
+    return gn_workspace(l, gn_bytes(l), clip ? NVDR_GN_ONE_CLIP : NVDR_GN_ONE_NORM);
 }
 
 #define NVDR_GN_STARTS 64
@@ -429,28 +501,51 @@ static int gn_parts(const GradList &l, int64_t bytes, double *part, GradLaunches
 }
 
 template <int P>
-static int gn_norm(const GradList &l, double max_norm, double *part, float *norm, float *factor, hipStream_t st)
+static int gn_norm(const GradList &l, double *part, const GradOut &out, hipStream_t st)
 {
+    const int64_t bytes = gn_bytes(l);
+    if (gn_one(l, bytes, NVDR_GN_ONE_NORM)) {
+        GradTable tab;
+        int64_t at = 0, left = bytes;
+        gn_fill(l, &at, &left, 1, tab);
+        grad_norm_one_kernel<P><<<1, NVDR_GN_ONE_BLOCK, 0, st>>>(tab, out);
+        NVDR_LAUNCH_CHECK();
+        return 0;
+    }
     GradLaunches g;
-    if (int r = gn_parts<P>(l, gn_bytes(l), part, g, st)) return r;
-    grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, max_norm, norm, factor);
+    if (int r = gn_parts<P>(l, bytes, part, g, st)) return r;
+    grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, out);
     NVDR_LAUNCH_CHECK();
     return 0;
+}
+
+static int gn_norm_typed(const GradList &l, int norm_type, double *part, const GradOut &out, hipStream_t st)
+{
+    return norm_type == NVDR_NORM_INF ? gn_norm<GN_INF>(l, part, out, st) : norm_type == NVDR_NORM_1 ? gn_norm<GN_ONE>(l, part, out, st) : gn_norm<GN_TWO>(l, part, out, st);
 }
 
 template <int P>
 static int gn_clip(const GradList &l, double max_norm, double *part, float *norm, float *factor, hipStream_t st)
 {
-    GradLaunches g;
     const int64_t bytes = gn_bytes(l);
+    GradTable tab;
+    if (gn_one(l, bytes, NVDR_GN_ONE_CLIP)) {
+        int64_t at = 0, left = bytes;
+        gn_fill(l, &at, &left, 1, tab);
+        grad_clip_one_kernel<P><<<1, NVDR_GN_ONE_BLOCK, 0, st>>>(tab, max_norm, norm);
+        NVDR_LAUNCH_CHECK();
+        return 0;
+    }
+    GradLaunches g;
     if (int r = gn_parts<P>(l, bytes, part, g, st)) return r;
     if (g.count != 1) {
-        grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, max_norm, norm, factor);
+        GradOut out = {};
+        out.max_norm = max_norm; out.norm = norm; out.factor = factor;
+        grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, out);
         NVDR_LAUNCH_CHECK();
     }
     const int n_part = g.count == 1 ? g.n_part : 0;
     const bool stream = bytes > NVDR_GN_KEEP;
-    GradTable tab;
     auto launch = [&](int64_t at, int64_t left, int64_t *behind, int64_t *after) -> bool {
         const unsigned blocks = gn_fill(l, &at, &left, stream ? NVDR_GN_STREAM_GRID : NVDR_GN_GRID, tab);
         if (blocks && stream) grad_scale_kernel<P, true><<<blocks, NVDR_GN_STREAM_BLOCK, 0, st>>>(tab, part, n_part, max_norm, norm, factor);
@@ -475,13 +570,30 @@ extern "C" int nvdr_grad_norm(const void *const *data, const int64_t *n, const u
 {
     NvdrRange range("nvdr_grad_norm");
     const GradList l = {data, n, type, scale, n_tensors};
-    if (int r = gn_check(l, max_norm, workspace, workspace_len, norm, "nvdr_grad_norm")) return r;
-    switch (norm_type) {
-    case NVDR_NORM_INF: return gn_norm<GN_INF>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
-    case NVDR_NORM_1: return gn_norm<GN_ONE>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
-    case NVDR_NORM_2: return gn_norm<GN_TWO>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
+    if (int r = gn_check(l, norm_type, max_norm, NVDR_GN_ONE_NORM, workspace, workspace_len, norm, "nvdr_grad_norm")) return r;
+    GradOut out = {};
+    out.max_norm = max_norm; out.norm = norm; out.factor = factor;
+    return gn_norm_typed(l, norm_type, workspace, out, (hipStream_t)stream);
+}
+
+int nvdr_adam_norm(const nvdr_adam_tensor *tensors, int n_tensors, int norm_type, double max_norm, double *workspace, int64_t workspace_len, float *norm,
+                   const AdamBegin &adam, hipStream_t stream)
+{
+    const void *data[NVDR_ADAM_MAX_TENSORS];
+    int64_t n[NVDR_ADAM_MAX_TENSORS];
+    uint8_t type[NVDR_ADAM_MAX_TENSORS];
+    float scale[NVDR_ADAM_MAX_TENSORS];
+    int m = 0;
+    for (int k = 0; k < n_tensors; ++k) {
+        if (tensors[k].frozen) continue;
+        data[m] = tensors[k].grad; n[m] = tensors[k].n; type[m] = GN_F32; scale[m] = tensors[k].grad_scale;
+        ++m;
     }
-    NVDR_REQUIRE(false, "nvdr_grad_norm: norm type %d", norm_type);
+    const GradList l = {data, n, type, scale, m};
+    if (int r = gn_check(l, norm_type, max_norm, NVDR_GN_ONE_NORM, workspace, workspace_len, norm, "nvdr_adam_step_clipped")) return r;
+    GradOut out = {};
+    out.max_norm = max_norm; out.norm = norm; out.adam = adam;
+    return gn_norm_typed(l, norm_type, workspace, out, stream);
 }
 
 extern "C" int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t *type, int64_t n_tensors, int norm_type, double max_norm, double *workspace,
@@ -489,13 +601,12 @@ extern "C" int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t
 {
     NvdrRange range("nvdr_grad_clip");
     const GradList l = {(const void *const *)data, n, type, nullptr, n_tensors};
-    if (int r = gn_check(l, max_norm, workspace, workspace_len, norm, "nvdr_grad_clip")) return r;
+    if (int r = gn_check(l, norm_type, max_norm, NVDR_GN_ONE_CLIP, workspace, workspace_len, norm, "nvdr_grad_clip")) return r;
     if (int r = gn_check_apart(l, "nvdr_grad_clip")) return r;
-    float *factor = (float *)(workspace + workspace_len - 1);
+    float *factor = workspace ? (float *)(workspace + workspace_len - 1) : nullptr;
     switch (norm_type) {
     case NVDR_NORM_INF: return gn_clip<GN_INF>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
     case NVDR_NORM_1: return gn_clip<GN_ONE>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
-    case NVDR_NORM_2: return gn_clip<GN_TWO>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
+    default: return gn_clip<GN_TWO>(l, max_norm, workspace, norm, factor, (hipStream_t)stream);
     }
-    NVDR_REQUIRE(false, "nvdr_grad_clip: norm type %d", norm_type);
 }

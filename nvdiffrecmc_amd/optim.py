@@ -9,6 +9,7 @@ device memory, so the launch can be captured in a HIP graph.
 import array
 import contextlib
 import math
+import struct
 
 import torch
 
@@ -49,8 +50,13 @@ def _gradients(tensors, what, grads=False, written=False):
         raise type(e)('%s: %s' % (what, e)) from None
 
 
-def _workspace(count, device):
-    return torch.empty(_lib.load().nvdr_grad_norm_workspace(count), dtype=torch.float64, device=device)
+def _workspace(n, types, clip, device):
+    """(address, doubles, owner) of the device memory a call needs, nothing for a short list."""
+    size = _lib.load().nvdr_grad_norm_workspace(n, types, len(types), clip)
+    if size == 0:
+        return None, 0, None
+    work = torch.empty(size, dtype=torch.float64, device=device)
+    return work.data_ptr(), size, work
 
 
 def _on(device_index):
@@ -72,9 +78,10 @@ def grad_norm(tensors, norm_type=2.0, scales=None):
     if device < 0:
         return torch.zeros(())
     with _on(device):
-        work, norm = _workspace(len(types), device), torch.empty((), dtype=torch.float32, device=device)
-        _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0] if scales else None, len(types), code, math.inf, work.data_ptr(),
-                                              work.numel(), norm.data_ptr(), None, _lib.stream_ptr()), 'grad_norm')
+        work, size, _owner = _workspace(n, types, 0, device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0] if scales else None, len(types), code, math.inf, work, size,
+                                              norm.data_ptr(), None, _lib.stream_ptr()), 'grad_norm')
     return norm
 
 
@@ -102,14 +109,17 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
                 raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
             reach += (size - 1) * stride
     with _on(device):
-        work, norm = _workspace(len(types), device), torch.empty((), dtype=torch.float32, device=device)
-        _lib.check(_lib.load().nvdr_grad_clip(data, n, types, len(types), code, max_norm, work.data_ptr(), work.numel(), norm.data_ptr(),
-                                              _lib.stream_ptr()), 'clip_grad_norm_')
+        work, size, _owner = _workspace(n, types, 1, device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        _lib.check(_lib.load().nvdr_grad_clip(data, n, types, len(types), code, max_norm, work, size, norm.data_ptr(), _lib.stream_ptr()), 'clip_grad_norm_')
         if copies:
             with torch.no_grad():
                 for g, copy in copies:
                     g.copy_(copy)
     return norm
+
+
+_ADAM_ROW = struct.Struct('=QQQQqfff4xQqQqfiQii').pack          # nvdr_adam_tensor (_lib.NvdrAdamTensor): filling its fields one by one costs 2 us a tensor
 
 
 class FusedAdam:
@@ -149,7 +159,10 @@ class FusedAdam:
         dev = self.params[0].device
         self._norm_out = torch.zeros(2, dtype=torch.float32, device=dev) if max_norm is not None else None       # norm, factor
         self._norm_view = self._norm_out[0] if max_norm is not None else None
-        self._norm_work = _workspace(len(self.params), dev) if max_norm is not None else None
+        self._norm_work = None
+        if max_norm is not None:        # (what the step begins with, and the parts of the norm: enough for any part of the tensors)
+            n, types = array.array('q', [p.numel() for p in self.params]).tobytes(), bytes(len(self.params))
+            self._norm_work = torch.empty(2 + _lib.load().nvdr_grad_norm_workspace(n, types, len(types), 0), dtype=torch.float64, device=dev)
         self.state = torch.zeros(8, dtype=torch.int32, device=self.params[0].device)     # steps taken, scratch, beta1^t, beta2^t (doubles)
 
     @property
@@ -162,8 +175,9 @@ class FusedAdam:
         return self._norm_view
 
     def measure_norm(self, grad_mult=1.0):
-        """The norm of this iteration's gradients into .grad_norm, and the factor of the updates that follow (max_norm).  step() calls it;
-        a caller that updates in subsets calls it once, when every gradient of the iteration is there, in front of the first subset."""
+        """The norm of this iteration's gradients into .grad_norm, and the factor of the updates that follow (max_norm).  step() of all tensors
+        does it itself; a caller that updates in subsets calls it once, when every gradient of the iteration is there, in front of the
+        first subset."""
         if self.max_norm is None:
             raise RuntimeError('FusedAdam.measure_norm: no max_norm was given')
         live = [i for i in range(len(self.params)) if float(self.lr_scales[i]) != 0.0]
@@ -173,8 +187,8 @@ class FusedAdam:
         scales = array.array('f', [float(self.grad_scales[i]) * float(grad_mult) for i in live])
         device, data, n, types, _copies = _gradients([self.params[i].grad for i in live], 'FusedAdam')
         with _on(self.state.get_device()):
-            _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0], len(types), self._norm_code, self.max_norm, self._norm_work.data_ptr(),
-                                                  self._norm_work.numel(), self._norm_out.data_ptr(), self._norm_out.data_ptr() + 4, _lib.stream_ptr()), 'grad_norm')
+            _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0], len(types), self._norm_code, self.max_norm, self._norm_work.data_ptr() + 16,
+                                                  self._norm_work.numel() - 2, self._norm_out.data_ptr(), self._norm_out.data_ptr() + 4, _lib.stream_ptr()), 'grad_norm')
         self._measured = True
 
     def zero_grad(self, set_to_none=True):
@@ -189,46 +203,48 @@ class FusedAdam:
         launch of an iteration but the last, nvdr_adam_step_partial); grad_mult: extra factor on the gradients of this launch (1 / world
         after a summing all-reduce).  With max_norm a launch of all tensors measures the norm first; subsets need measure_norm() before the
         first of them."""
-        factor = None
-        if self.max_norm is not None:
-            if subset is None:
-                self.measure_norm(grad_mult)
-            elif not self._measured:
-                raise RuntimeError('FusedAdam.step: with max_norm, measure_norm() comes before the first subset of an iteration')
-            factor = self._norm_out.data_ptr() + 4
-            self._measured = not advance
-        idx = list(range(len(self.params))) if subset is None else list(subset)
-        tab = (_lib.NvdrAdamTensor * len(idx))()
-        keep = []
-        for j, i in enumerate(idx):
+        idx = range(len(self.params)) if subset is None else list(subset)
+        rows, keep = [], []
+        for i in idx:
             p = self.params[i]
-            if p.grad is None:
+            g = p.grad
+            if g is None:
                 raise RuntimeError('FusedAdam.step: parameter %d has no gradient' % i)
-            if self.zero_grad_after[i] and not p.grad.is_contiguous():
-                # a copy would be zeroed instead of the buffer the producer scatter-adds into
-                raise RuntimeError('FusedAdam.step: zero_grad needs a contiguous .grad for parameter %d (the persistent scatter-add buffer itself)' % i)
-            g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
-            keep.append(g)
+            if not g.is_contiguous():
+                if self.zero_grad_after[i]:
+                    # a copy would be zeroed instead of the buffer the producer scatter-adds into
+                    raise RuntimeError('FusedAdam.step: zero_grad needs a contiguous .grad for parameter %d (the persistent scatter-add buffer itself)' % i)
+                g = g.contiguous()
+                keep.append(g)
             lo, hi, lo_vec, hi_vec = -math.inf, math.inf, None, None
-            if self.clamps[i] is not None:
-                c = self.clamps[i]
+            c = self.clamps[i]
+            if c is not None:
                 lo = -math.inf if c[0] is None else float(c[0])
                 hi = math.inf if c[1] is None else float(c[1])
                 lo_vec = c[2] if len(c) > 2 else None
                 hi_vec = c[3] if len(c) > 3 else None
-            t = tab[j]
-            t.param, t.grad, t.exp_avg, t.exp_avg_sq = p.data_ptr(), g.data_ptr(), self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr()
-            t.n = p.numel()
-            t.grad_scale, t.lo, t.hi = float(self.grad_scales[i]) * float(grad_mult), lo, hi
-            t.lo_vec = lo_vec.data_ptr() if lo_vec is not None else None
-            t.lo_vec_n = lo_vec.numel() if lo_vec is not None else 0
-            t.hi_vec = hi_vec.data_ptr() if hi_vec is not None else None
-            t.hi_vec_n = hi_vec.numel() if hi_vec is not None else 0
             # lr_scales[i] == 0 freezes the tensor (the C block's lr_scale 0 means "the plain rate": a zero-initialised block trains)
-            t.lr_scale, t.normalize3 = float(self.lr_scales[i]) or 1.0, int(bool(self.normalize3[i]))
-            t.frozen = int(float(self.lr_scales[i]) == 0.0)
-            t.active = self.active[i].data_ptr() if self.active[i] is not None else None
-            t.zero_grad = int(bool(self.zero_grad_after[i] and self.active[i] is not None))
-        with torch.no_grad(), _on(self.state.get_device()):
-            _lib.check(_lib.load().nvdr_adam_step_clipped(tab, len(idx), self.lr, self.betas[0], self.betas[1], self.eps,
-                                                          _lib.ptr(self.state), int(bool(advance)), factor, _lib.stream_ptr()), 'adam_step')
+            rate, active = float(self.lr_scales[i]), self.active[i]
+            rows.append(_ADAM_ROW(p.data_ptr(), g.data_ptr(), self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr(), p.numel(),
+                                  float(self.grad_scales[i]) * float(grad_mult), lo, hi,
+                                  lo_vec.data_ptr() if lo_vec is not None else 0, lo_vec.numel() if lo_vec is not None else 0,
+                                  hi_vec.data_ptr() if hi_vec is not None else 0, hi_vec.numel() if hi_vec is not None else 0,
+                                  rate or 1.0, bool(self.normalize3[i]), active.data_ptr() if active is not None else 0,
+                                  bool(self.zero_grad_after[i]) and active is not None, rate == 0.0))
+        tab, lib, state = b''.join(rows), _lib.load(), self.state.data_ptr()
+        hyper = (self.lr, self.betas[0], self.betas[1], self.eps)
+        with _on(self.state.get_device()):
+            if self.max_norm is not None and subset is None and advance:
+                _lib.check(lib.nvdr_adam_step_clipped(tab, len(rows), *hyper, state, self._norm_code, self.max_norm, self._norm_work.data_ptr(),
+                                                      self._norm_work.numel(), self._norm_out.data_ptr(), _lib.stream_ptr()), 'adam_step')
+                self._measured = False
+                return
+            factor = None
+            if self.max_norm is not None:
+                if subset is None:
+                    self.measure_norm(grad_mult)
+                elif not self._measured:
+                    raise RuntimeError('FusedAdam.step: with max_norm, measure_norm() comes before the first subset of an iteration')
+                factor = self._norm_out.data_ptr() + 4
+                self._measured = not advance
+            _lib.check(lib.nvdr_adam_step_factor(tab, len(rows), *hyper, state, bool(advance), factor, _lib.stream_ptr()), 'adam_step')

@@ -443,7 +443,7 @@ def test_clipped_step_equals_scaled_gradients(dev):
         for x, y, g in zip(a.params, b.params, h):
             x.grad, y.grad = g.to(dev), (g * 0.25).to(dev)
         a.step()
-        assert a._norm_out[1].item() == 0.25
+        assert a._norm_work.view(F32)[0].item() == 0.25                     # (what the step begins with: factor, step size, ...)
         b.step()
     for i in range(len(SHAPES)):
         assert torch.equal(a.params[i], b.params[i]) and torch.equal(a.exp_avg[i], b.exp_avg[i]) and torch.equal(a.exp_avg_sq[i], b.exp_avg_sq[i]), i

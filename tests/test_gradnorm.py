@@ -50,8 +50,8 @@ def _call(entry, data, n, types, max_norm=1.0, norm_type=2, workspace=None, out=
     """The entry on host lists (addresses are never dereferenced: every call here is refused)."""
     lib = _lib.load()
     d, c = array.array('Q', data).tobytes(), array.array('q', n).tobytes()
-    need = lib.nvdr_grad_norm_workspace(len(n))
-    ws = torch.empty(need if workspace is None else workspace, dtype=torch.float64)
+    need = lib.nvdr_grad_norm_workspace(c, bytes(types), len(n), int(entry == 'nvdr_grad_clip'))
+    ws = torch.empty(max(need, 1) if workspace is None else workspace, dtype=torch.float64)
     o = torch.empty(2)
     args = [d, c, bytes(types)] + ([scale] if entry == 'nvdr_grad_norm' else [])
     args += [len(n), norm_type, max_norm, ws.data_ptr(), ws.numel(), o.data_ptr() if out else None] + ([None] if entry == 'nvdr_grad_norm' else []) + [None]
@@ -69,7 +69,8 @@ def test_entries_refuse_bad_arguments(entry):
         (dict(data=[0], n=[4], types=[0]), 'no memory'),
         (dict(data=[A + 2], n=[4], types=[0]), 'aligned'),
         (dict(data=[A + 1], n=[4], types=[1]), 'aligned'),
-        (dict(data=[A], n=[4], types=[0], workspace=8), 'workspace'),
+        (dict(data=[A], n=[1 << 30], types=[0], workspace=8), 'workspace'),
+        (dict(data=[A] * 9, n=[0] * 9, types=[0] * 9, workspace=8), 'workspace'),
         (dict(data=[A], n=[4], types=[0], out=False), 'norm'),
         (dict(data=[A], n=[4], types=[0], max_norm=-1.0), 'max_norm'),
         (dict(data=[A], n=[4], types=[0], max_norm=math.nan), 'max_norm'),
@@ -93,10 +94,16 @@ def test_clip_refuses_gradients_that_share_memory():
         assert rc == -1 and 'share memory' in msg, (data, n, rc, msg)
 
 
-def test_workspace_grows_with_the_list():
+def test_workspace_of_a_list():
     lib = _lib.load()
-    sizes = [lib.nvdr_grad_norm_workspace(n) for n in (0, 1, 160, 161, 1000)]
-    assert sizes[0] > 0 and sizes == sorted(sizes) and sizes[1] == sizes[2] < sizes[3] < sizes[4]
+
+    def need(sizes, clip=0, t=0):
+        return lib.nvdr_grad_norm_workspace(array.array('q', sizes).tobytes(), bytes([t]) * len(sizes), len(sizes), clip)
+    assert need([]) == need([1]) == need([0, 7]) == need([1], clip=1) == 0             # a short list: one workgroup, no parts
+    assert need([1 << 30]) > 512 and need([1 << 30], clip=1) > 512
+    assert need([1] * 9) > 512                                                          # many tensors are no short list
+    assert need([1] * 160) == need([1] * 9) < need([1] * 161) < need([1] * 1000)
+    assert need([1 << 16]) >= need([1 << 15]) and need([1 << 16], t=1) <= need([1 << 16])
 
 
 def test_a_missing_extension_is_an_error(monkeypatch):
@@ -109,5 +116,21 @@ def test_a_missing_extension_is_an_error(monkeypatch):
 
 def test_adam_entry_refuses_without_a_launch():
     lib = _lib.load()
-    rc = lib.nvdr_adam_step_clipped(None, 0, ctypes.c_double(1e-3), 0.9, 0.999, 1e-8, None, 1, None, None)
-    assert rc == -1 and b'NULL' in lib.nvdr_last_error()
+    assert lib.nvdr_adam_step_factor(None, 0, 1e-3, 0.9, 0.999, 1e-8, None, 1, None, None) == -1 and b'NULL' in lib.nvdr_last_error()
+    assert lib.nvdr_adam_step_clipped(None, 0, 1e-3, 0.9, 0.999, 1e-8, None, 2, 1.0, None, 0, None, None) == -1 and b'NULL' in lib.nvdr_last_error()
+    A = 1 << 20
+    row = optim._ADAM_ROW(A, A, A, A, 4, 1.0, -math.inf, math.inf, 0, 0, 0, 0, 1.0, 0, 0, 0, 0)
+    ws, norm = torch.empty(8, dtype=torch.float64), torch.empty(1)
+    at = ws.data_ptr() + (-ws.data_ptr()) % 16
+    for kw, word in ((dict(workspace=None), b'workspace'), (dict(workspace=at + 8), b'workspace'), (dict(size=1), b'workspace'), (dict(norm=None), b'norm'),
+                     (dict(norm_type=5), b'norm type'), (dict(max_norm=-1.0), b'max_norm'), (dict(lr=-1.0), b'hyper')):
+        a = dict(dict(lr=1e-3, norm_type=2, max_norm=1.0, workspace=at, size=4, norm=norm.data_ptr()), **kw)
+        rc = lib.nvdr_adam_step_clipped(row, 1, a['lr'], 0.9, 0.999, 1e-8, A, a['norm_type'], a['max_norm'], a['workspace'], a['size'], a['norm'], None)
+        assert rc == -1 and word in lib.nvdr_last_error(), (kw, rc, lib.nvdr_last_error())
+
+
+def test_the_packed_row_is_the_structure():
+    row = optim._ADAM_ROW(1, 2, 3, 4, 5, 6.0, 7.0, 8.0, 9, 10, 11, 12, 13.0, 14, 15, 16, 17)
+    t = _lib.NvdrAdamTensor.from_buffer_copy(row)
+    assert len(row) == ctypes.sizeof(_lib.NvdrAdamTensor)
+    assert [getattr(t, n) for n, _ in _lib.NvdrAdamTensor._fields_] == list(range(1, 18))

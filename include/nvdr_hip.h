@@ -502,8 +502,8 @@ int nvdr_adam_step_clipped(const nvdr_adam_tensor *tensors, int n_tensors, doubl
  *     factor = min(1, max_norm / (norm + 1e-6)); one for an infinite max_norm
  * data[k]: n[k] contiguous elements of type[k] in any mixture, aligned to their own size; n[k] = 0 is skipped.  scale: NULL for ones.  The
  * four lists live in HOST memory and are read before the call returns (a captured graph keeps them).  Sums in fp64, in an order that depends
- * on sizes and alignment only.  workspace: nvdr_grad_norm_workspace(n, type, n_tensors, clip) doubles of device memory (none for a short list,
- * which one workgroup takes), 8-byte aligned, nothing to initialise; launches that may run at the same time need one each.  norm, factor: one float each in device memory (factor may be NULL).
+ * on sizes and alignment only.  workspace: nvdr_grad_norm_workspace(n, type, n_tensors, clip) doubles of device memory (none for a short list
+ * that is clipped, which one workgroup does), 8-byte aligned, nothing to initialise; launches that may run at the same time need one each.  norm, factor: one float each in device memory (factor may be NULL).
  * nvdr_grad_norm leaves the gradients alone; nvdr_grad_clip multiplies them by the factor in place (computed in fp32, one rounding to the
  * element's type) and writes nothing when the factor is one.  Gradients of nvdr_grad_clip must not share memory. */
 enum { NVDR_GRAD_F32 = 0, NVDR_GRAD_BF16 = 1, NVDR_GRAD_F16 = 2 };

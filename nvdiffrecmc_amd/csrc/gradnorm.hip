@@ -31,6 +31,8 @@
 // scaling and for whoever reads the gradients next.
 #include <stdlib.h>
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 
 #include "common.h"
 #include "gradnorm.h"
@@ -44,10 +46,10 @@
 #define NVDR_GN_CHUNK 4096              // bytes
 #define NVDR_GN_RUN (128 << 10)         // bytes
 #define NVDR_GN_KEEP (160ll << 20)      // bytes that stay in the last-level cache (256 MB) from one pass to the next: 96 to 256 MB within 2 %
-#define NVDR_GN_ONE_BLOCK 1024          // a short list: one workgroup does all of it
+#define NVDR_GN_ONE_BLOCK 1024          // a short list: one workgroup clips all of it
 #define NVDR_GN_ONE_TENSORS 8
-#define NVDR_GN_ONE_NORM (256 << 10)    // bytes
 #define NVDR_GN_ONE_CLIP (64 << 10)     // bytes
+#define NVDR_GN_PATIENCE (1 << 24)      // polls after which a workgroup no longer waits for another (seconds; nothing reaches it)
 #define NVDR_GN_EPS 1e-6
 
 enum { GN_INF = 0, GN_ONE = 1, GN_TWO = 2 };                // the kernels' norm types
@@ -197,14 +199,6 @@ __device__ __forceinline__ double gn_sum_runs(const GradTable &tab)
     return sum;
 }
 
-template <int P>
-__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_part_kernel(GradTable tab, double *__restrict__ part)
-{
-    __shared__ double lds[NVDR_GN_BLOCK / 64];
-    const double sum = gn_block_join<P>(gn_sum_runs<P, NVDR_GN_BLOCK>(tab), lds);
-    if (threadIdx.x == 0) part[blockIdx.x] = sum;
-}
-
 // ---- the norm of the parts, and the factor -----------------------------------------------------------------------------------------
 template <int P>
 __device__ __forceinline__ double gn_root(double v) { return P == GN_TWO ? sqrt(v) : v; }
@@ -246,21 +240,58 @@ __device__ __forceinline__ void gn_finish(double norm, const GradOut &o)
     }
 }
 
-template <int P>
-__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_final_kernel(const double *__restrict__ part, int n_part, GradOut out)
+// The parts of one table.  FINISH, in the last launch of a norm: its first workgroup waits for the others and writes the norm, `before` parts
+// of earlier launches included, so that no kernel has to follow for it (a launch costs 4 us, the wait about 1).
+//
+// The wait.  Every other workgroup stores its part as two words, its bits under one key each, and the first one polls both until they open to the
+// same bits.  Nobody waits for the first workgroup, so the others end whatever it does, and its wait ends with them.  Stores and loads go
+// past the caches of the XCDs; nothing else is published, so no cache has to be written back or emptied for it (with a release and a tag
+// behind the part, every workgroup wrote back what kernels before it had left in its L2: 25 instead of 17 us in front of an Adam step).
+// The memory needs no clearing: a pair of keys belongs to one call only -- the host makes them from a counter, scrambled -- so that what
+// another call or another tensor has left there does not open, and the first workgroup erases the words it has read, so that a captured
+// launch finds none of its own when it is replayed.
+struct GradKeys {
+    unsigned long long a, b;
+};
+
+template <int P, bool FINISH>
+__global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_kernel(GradTable tab, double *part, unsigned long long *words, GradKeys keys, int before, GradOut out)
 {
     __shared__ double lds[NVDR_GN_BLOCK / 64];
-    const double norm = gn_total<P>(part, n_part, lds);
-    if (threadIdx.x == 0) gn_finish(norm, out);
-}
-
-// a short list: all of it by one workgroup, in one launch and without parts
-template <int P>
-__global__ void __launch_bounds__(NVDR_GN_ONE_BLOCK) grad_norm_one_kernel(GradTable tab, GradOut out)
-{
-    __shared__ double lds[NVDR_GN_ONE_BLOCK / 64];
-    const double norm = gn_root<P>(gn_block_join<P>(gn_sum_runs<P, NVDR_GN_ONE_BLOCK>(tab), lds));
-    if (threadIdx.x == 0) gn_finish(norm, out);
+    const double sum = gn_block_join<P>(gn_sum_runs<P, NVDR_GN_BLOCK>(tab), lds);
+    if (!FINISH) {
+        if (threadIdx.x == 0) part[before + blockIdx.x] = sum;
+        return;
+    }
+    if (blockIdx.x != 0) {
+        if (threadIdx.x == 0) {
+            const unsigned long long bits = (unsigned long long)__double_as_longlong(sum);
+            __hip_atomic_store(words + 2 * blockIdx.x, bits ^ keys.a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(words + 2 * blockIdx.x + 1, bits ^ keys.b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        return;
+    }
+    double v = 0.0;
+    for (int i = threadIdx.x; i < before + (int)gridDim.x; i += NVDR_GN_BLOCK) {
+        double x = sum;
+        if (i < before) x = part[i];
+        else if (i > before) {
+            unsigned long long *w = words + 2 * (i - before), p, q;
+            int left = NVDR_GN_PATIENCE;
+            for (;;) {
+                p = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ^ keys.a;
+                q = __hip_atomic_load(w + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ^ keys.b;
+                if (p == q || --left == 0) break;
+                __builtin_amdgcn_s_sleep(1);
+            }
+            x = p == q ? __longlong_as_double((long long)p) : (double)__builtin_nanf("");
+            __hip_atomic_store(w, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(w + 1, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        v = gn_join<P>(v, x);
+    }
+    v = gn_root<P>(gn_block_join<P>(v, lds));
+    if (threadIdx.x == 0) gn_finish(v, out);
 }
 
 // ---- scaling -------------------------------------------------------------------------------------------------------------------------
@@ -328,8 +359,7 @@ __device__ __forceinline__ void gn_scale_runs(const GradTable &tab, float f)
     }
 }
 
-// n_part > 0: every workgroup adds the parts up itself, in the same order (a launch less than a kernel of its own for it), and the first one
-// writes the norm; n_part = 0: the factor is there.  NT: the list is longer than what stays in the cache.
+// n_part > 0: every workgroup adds the parts up itself, in the same order, and the first one writes the norm; n_part = 0: the factor is there.  NT: the list is longer than what stays in the cache.
 template <int P, bool NT>
 __global__ void __launch_bounds__(NT ? NVDR_GN_STREAM_BLOCK : NVDR_GN_BLOCK)
 grad_scale_kernel(GradTable tab, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm, const float *__restrict__ factor)
@@ -374,16 +404,14 @@ static int64_t gn_bytes(const GradList &l)
     return bytes;
 }
 
-static bool gn_one(const GradList &l, int64_t bytes, int64_t most) { return l.count <= NVDR_GN_ONE_TENSORS && bytes <= most; }
+static bool gn_one(const GradList &l, int64_t bytes) { return l.count <= NVDR_GN_ONE_TENSORS && bytes <= NVDR_GN_ONE_CLIP; }
 
-static int64_t gn_workspace(const GradList &l, int64_t bytes, int64_t most)
-{
-    if (gn_one(l, bytes, most)) return 0;
-    // (a launch ends with the list or with a full table; the split by the number of chunks needs more than 2^31 of them, 8 TB)
-    return ((l.count + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID + 1;      // (the last: the factor of nvdr_grad_clip)
-}
+// in doubles: the parts, the words of the last launch, the factor of nvdr_grad_clip.  (A launch ends with the list or with a full table; the split by
+// the number of chunks needs more than 2^31 of them, 8 TB.)
+static int64_t gn_part_room(int64_t count) { return ((count + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID; }
+static int64_t gn_workspace(const GradList &l, bool clip) { return clip && gn_one(l, gn_bytes(l)) ? 0 : gn_part_room(l.count) + 2 * NVDR_GN_GRID + 1; }
 
-static int gn_check(const GradList &l, int norm_type, double max_norm, int64_t most, const double *workspace, int64_t workspace_len, const float *norm, const char *who)
+static int gn_check(const GradList &l, int norm_type, double max_norm, bool clip, const double *workspace, int64_t workspace_len, const float *norm, const char *who)
 {
     NVDR_REQUIRE(l.count >= 0 && l.count < (1ll << 24), "%s: %lld tensors", who, (long long)l.count);
     NVDR_REQUIRE(l.count == 0 || (l.data && l.n && l.type), "%s: NULL argument", who);
@@ -396,7 +424,7 @@ static int gn_check(const GradList &l, int norm_type, double max_norm, int64_t m
         NVDR_REQUIRE(l.n[k] == 0 || (l.data[k] && (uintptr_t)l.data[k] < (1ull << 62)), "%s: tensor %lld has no memory", who, (long long)k);
         NVDR_REQUIRE((uintptr_t)l.data[k] % (uintptr_t)gn_size(l.type[k]) == 0, "%s: tensor %lld is not aligned to its elements", who, (long long)k);
     }
-    const int64_t need = gn_workspace(l, gn_bytes(l), most);
+    const int64_t need = gn_workspace(l, clip);
     NVDR_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 7) == 0 && workspace_len >= need), "%s: an 8-byte aligned workspace of %lld doubles is needed, there are %lld",
                  who, (long long)need, (long long)(workspace ? workspace_len : 0));
     return 0;
@@ -473,7 +501,7 @@ extern "C" int64_t nvdr_grad_norm_workspace(const int64_t *n, const uint8_t *typ
 {
     const GradList l = {nullptr, n, type, nullptr, n_tensors};
     if (n_tensors < 0 || (n_tensors && (!n || !type))) return 0;
-    return gn_workspace(l, gn_bytes(l), clip ? NVDR_GN_ONE_CLIP : NVDR_GN_ONE_NORM);
+    return gn_workspace(l, clip != 0);
 }
 
 #define NVDR_GN_STARTS 64
@@ -483,40 +511,47 @@ struct GradLaunches {
     int n_part = 0;
 };
 
-template <int P>
-static int gn_parts(const GradList &l, int64_t bytes, double *part, GradLaunches &g, hipStream_t st)
+// keys of its own for every norm: splitmix64 of a counter, a bijection
+static GradKeys gn_keys()
 {
+    static std::atomic<unsigned long long> counter{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() << 20};
+    const unsigned long long at = counter.fetch_add(2, std::memory_order_relaxed);
+    auto mix = [](unsigned long long z) {
+        z *= 0x9e3779b97f4a7c15ull;
+        z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+        z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+        return z ^ (z >> 31);
+    };
+    return {mix(at), mix(at + 1)};          // (of two different counts: never equal, so that erased words do not open)
+}
+
+// the launches of the norm; finish: the last one writes it
+template <int P>
+static int gn_parts(const GradList &l, int64_t bytes, double *part, bool finish, const GradOut &out, GradLaunches &g, hipStream_t st)
+{
+    unsigned long long *words = (unsigned long long *)(part + gn_part_room(l.count));
     GradTable tab;
     int64_t at = 0, left = bytes;
-    for (;;) {
+    do {
         if (g.count < NVDR_GN_STARTS) { g.start[g.count] = at; g.left[g.count] = left; }
-        const unsigned blocks = gn_fill(l, &at, &left, NVDR_GN_GRID, tab);
-        if (!blocks) break;
-        grad_norm_part_kernel<P><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part + g.n_part);
+        unsigned blocks = gn_fill(l, &at, &left, NVDR_GN_GRID, tab);
+        while (at < l.count && l.n[at] == 0) ++at;                  // (nothing but empty tensors left: this is the last launch)
+        if (finish && at == l.count) {
+            if (!blocks) blocks = 1;                                // (nothing at all: a norm of zero)
+            grad_norm_kernel<P, true><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part, words, gn_keys(), g.n_part, out);
+        } else if (blocks) grad_norm_kernel<P, false><<<blocks, NVDR_GN_BLOCK, 0, st>>>(tab, part, words, GradKeys{}, g.n_part, out);
         NVDR_LAUNCH_CHECK();
         g.n_part += (int)blocks;
         ++g.count;
-    }
+    } while (at < l.count);
     return 0;
 }
 
 template <int P>
 static int gn_norm(const GradList &l, double *part, const GradOut &out, hipStream_t st)
 {
-    const int64_t bytes = gn_bytes(l);
-    if (gn_one(l, bytes, NVDR_GN_ONE_NORM)) {
-        GradTable tab;
-        int64_t at = 0, left = bytes;
-        gn_fill(l, &at, &left, 1, tab);
-        grad_norm_one_kernel<P><<<1, NVDR_GN_ONE_BLOCK, 0, st>>>(tab, out);
-        NVDR_LAUNCH_CHECK();
-        return 0;
-    }
     GradLaunches g;
-    if (int r = gn_parts<P>(l, bytes, part, g, st)) return r;
-    grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, out);
-    NVDR_LAUNCH_CHECK();
-    return 0;
+    return gn_parts<P>(l, gn_bytes(l), part, true, out, g, st);
 }
 
 static int gn_norm_typed(const GradList &l, int norm_type, double *part, const GradOut &out, hipStream_t st)
@@ -529,22 +564,20 @@ static int gn_clip(const GradList &l, double max_norm, double *part, float *norm
 {
     const int64_t bytes = gn_bytes(l);
     GradTable tab;
-    if (gn_one(l, bytes, NVDR_GN_ONE_CLIP)) {
+    if (gn_one(l, bytes)) {
         int64_t at = 0, left = bytes;
         gn_fill(l, &at, &left, 1, tab);
         grad_clip_one_kernel<P><<<1, NVDR_GN_ONE_BLOCK, 0, st>>>(tab, max_norm, norm);
         NVDR_LAUNCH_CHECK();
         return 0;
     }
+    // one table: the scaling adds the parts up itself; several, or nothing to scale: the last launch of the norm leaves the norm and the factor
+    const bool finish = l.count > NVDR_GN_TENSORS || bytes == 0;
     GradLaunches g;
-    if (int r = gn_parts<P>(l, bytes, part, g, st)) return r;
-    if (g.count != 1) {
-        GradOut out = {};
-        out.max_norm = max_norm; out.norm = norm; out.factor = factor;
-        grad_norm_final_kernel<P><<<1, NVDR_GN_BLOCK, 0, st>>>(part, g.n_part, out);
-        NVDR_LAUNCH_CHECK();
-    }
-    const int n_part = g.count == 1 ? g.n_part : 0;
+    GradOut out = {};
+    out.max_norm = max_norm; out.norm = norm; out.factor = factor;
+    if (int r = gn_parts<P>(l, bytes, part, finish, out, g, st)) return r;
+    const int n_part = finish ? 0 : g.n_part;
     const bool stream = bytes > NVDR_GN_KEEP;
     auto launch = [&](int64_t at, int64_t left, int64_t *behind, int64_t *after) -> bool {
         const unsigned blocks = gn_fill(l, &at, &left, stream ? NVDR_GN_STREAM_GRID : NVDR_GN_GRID, tab);
@@ -561,7 +594,7 @@ static int gn_clip(const GradList &l, double max_norm, double *part, float *norm
         NVDR_LAUNCH_CHECK();
         if (k == known - 1) { at = a; left = b; }
     }
-    while (known && launch(at, left, &at, &left)) NVDR_LAUNCH_CHECK();
+    while (launch(at, left, &at, &left)) NVDR_LAUNCH_CHECK();
     return 0;
 }
 
@@ -570,7 +603,7 @@ extern "C" int nvdr_grad_norm(const void *const *data, const int64_t *n, const u
 {
     NvdrRange range("nvdr_grad_norm");
     const GradList l = {data, n, type, scale, n_tensors};
-    if (int r = gn_check(l, norm_type, max_norm, NVDR_GN_ONE_NORM, workspace, workspace_len, norm, "nvdr_grad_norm")) return r;
+    if (int r = gn_check(l, norm_type, max_norm, false, workspace, workspace_len, norm, "nvdr_grad_norm")) return r;
     GradOut out = {};
     out.max_norm = max_norm; out.norm = norm; out.factor = factor;
     return gn_norm_typed(l, norm_type, workspace, out, (hipStream_t)stream);
@@ -590,7 +623,7 @@ int nvdr_adam_norm(const nvdr_adam_tensor *tensors, int n_tensors, int norm_type
         ++m;
     }
     const GradList l = {data, n, type, scale, m};
-    if (int r = gn_check(l, norm_type, max_norm, NVDR_GN_ONE_NORM, workspace, workspace_len, norm, "nvdr_adam_step_clipped")) return r;
+    if (int r = gn_check(l, norm_type, max_norm, false, workspace, workspace_len, norm, "nvdr_adam_step_clipped")) return r;
     GradOut out = {};
     out.max_norm = max_norm; out.norm = norm; out.adam = adam;
     return gn_norm_typed(l, norm_type, workspace, out, stream);
@@ -601,7 +634,7 @@ extern "C" int nvdr_grad_clip(void *const *data, const int64_t *n, const uint8_t
 {
     NvdrRange range("nvdr_grad_clip");
     const GradList l = {(const void *const *)data, n, type, nullptr, n_tensors};
-    if (int r = gn_check(l, norm_type, max_norm, NVDR_GN_ONE_CLIP, workspace, workspace_len, norm, "nvdr_grad_clip")) return r;
+    if (int r = gn_check(l, norm_type, max_norm, true, workspace, workspace_len, norm, "nvdr_grad_clip")) return r;
     if (int r = gn_check_apart(l, "nvdr_grad_clip")) return r;
     float *factor = workspace ? (float *)(workspace + workspace_len - 1) : nullptr;
     switch (norm_type) {

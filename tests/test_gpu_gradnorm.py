@@ -58,6 +58,9 @@ def params_of(grads):
 
 LISTS = {
     'one': [1],
+    'many empties': [0] * 12,
+    'empties behind a full table': [3] * 160 + [0] * 300,
+    'one behind a full table and empties': [3] * 160 + [0] * 300 + [5],
     'empty': [0],
     'empties between': [0, 5, 0, 0, 70000, 0],
     'around a vector': [2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 33],

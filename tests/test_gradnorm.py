@@ -99,11 +99,11 @@ def test_workspace_of_a_list():
 
     def need(sizes, clip=0, t=0):
         return lib.nvdr_grad_norm_workspace(array.array('q', sizes).tobytes(), bytes([t]) * len(sizes), len(sizes), clip)
-    assert need([]) == need([1]) == need([0, 7]) == need([1], clip=1) == 0             # a short list: one workgroup, no parts
-    assert need([1 << 30]) > 512 and need([1 << 30], clip=1) > 512
-    assert need([1] * 9) > 512                                                          # many tensors are no short list
+    assert need([1], clip=1) == need([0, 7], clip=1) == need([], clip=1) == 0          # clipped by one workgroup
+    assert need([1 << 30]) == need([1]) >= need([]) > 512 and need([1 << 30], clip=1) == need([1 << 30])
+    assert need([1] * 9, clip=1) > 512                                                  # many tensors are no short list
     assert need([1] * 160) == need([1] * 9) < need([1] * 161) < need([1] * 1000)
-    assert need([1 << 16]) >= need([1 << 15]) and need([1 << 16], t=1) <= need([1 << 16])
+    assert need([1 << 16], clip=1, t=1) <= need([1 << 16], clip=1)
 
 
 def test_a_missing_extension_is_an_error(monkeypatch):

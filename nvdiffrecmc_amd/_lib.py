@@ -256,7 +256,7 @@ def check(rc, what):
 
 def stream_ptr():
     # (the handle alone: building a torch.cuda.Stream object for it costs 2.8 us a call)
-    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ptr(t):

@@ -55,14 +55,16 @@
 enum { GN_INF = 0, GN_ONE = 1, GN_TWO = 2 };                // the kernels' norm types
 enum { GN_F32 = NVDR_GRAD_F32, GN_BF16 = NVDR_GRAD_BF16, GN_F16 = NVDR_GRAD_F16 };
 
+// (what a workgroup asks for first lies in front, within one load)
 struct GradTable {
-    uint64_t data[NVDR_GN_TENSORS];             // address, the type in the upper two bits
-    int64_t n[NVDR_GN_TENSORS];                 // elements, never zero
-    uint32_t first[NVDR_GN_TENSORS + 1];        // chunks in front of the tensor
-    float scale[NVDR_GN_TENSORS];
     int n_tensors;
+    uint32_t chunks;
     uint32_t run;                               // chunks that a workgroup takes at a time
     uint32_t kept;                              // chunks from here on are loaded to stay in the last-level cache
+    uint32_t first[NVDR_GN_TENSORS + 8];        // chunks in front of the tensor; from n_tensors on: all of them
+    float scale[NVDR_GN_TENSORS];
+    uint64_t data[NVDR_GN_TENSORS];             // address, the type in the upper two bits
+    int64_t n[NVDR_GN_TENSORS];                 // elements, never zero
 };
 static_assert(sizeof(GradTable) <= 3900, "the kernel arguments have to fit 4 KB");
 
@@ -118,9 +120,16 @@ __device__ __forceinline__ double gn_block_join(double v, double *lds)
 }
 
 // ---- which part of which tensor ----------------------------------------------------------------------------------------------------
-// the tensor that chunk c falls into: the lanes compare 64 entries at a time (one round trip instead of a search's seven)
+// the tensor that chunk c falls into: of a few all entries are compared, of more 64 at a time by the lanes (one round trip each; a search would
+// take seven)
 __device__ __forceinline__ int gn_find(const GradTable &tab, uint32_t c)
 {
+    if (tab.n_tensors <= 8) {
+        int at = 0;
+#pragma unroll
+        for (int q = 1; q < 8; ++q) at += tab.first[q] <= c ? 1 : 0;
+        return at;
+    }
     const int lane = threadIdx.x & 63;
     int at = -1;
     for (int q = 0; q < tab.n_tensors; q += 64)
@@ -177,7 +186,7 @@ __device__ __forceinline__ double gn_sum_typed(const char *p, int type, int64_t 
 template <int P, int BLOCK>
 __device__ __forceinline__ double gn_sum_runs(const GradTable &tab)
 {
-    const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, kept = tab.kept;
+    const uint32_t chunks = tab.chunks, run = tab.run, kept = tab.kept;
     double sum = 0.0;
     for (uint64_t r = (uint64_t)blockIdx.x * run; r < chunks; r += (uint64_t)gridDim.x * run) {
         uint32_t c = (uint32_t)r;
@@ -225,17 +234,15 @@ struct GradOut {
     AdamBegin adam;             // adam.state: NULL for none
 };
 
-// what one thread writes when the norm is known.  In front of an Adam step also what that needs of its counter, which moves here: the
-// update reads no state, and no launch behind it is needed to move it
-__device__ __forceinline__ void gn_finish(double norm, const GradOut &o)
+// What one thread writes when the norm is known.  In front of an Adam step also what that needs of its counter, which moves here: the
+// update reads no state, and no launch behind it is needed to move it.  (`step`: adam_begin, computed where it costs no time.)
+__device__ __forceinline__ void gn_finish(double norm, const GradOut &o, AdamStep step)
 {
-    const float f = gn_factor(norm, o.max_norm);
+    step.factor = gn_factor(norm, o.max_norm);
     *o.norm = (float)norm;
-    if (o.factor) *o.factor = f;
+    if (o.factor) *o.factor = step.factor;
     if (o.adam.state) {
-        AdamStep s = adam_begin(o.adam.state, o.adam.lr, o.adam.beta1, o.adam.beta2);
-        s.factor = f;
-        *o.adam.step = s;
+        *o.adam.step = step;
         adam_advance(o.adam.state, o.adam.beta1, o.adam.beta2);
     }
 }
@@ -271,6 +278,8 @@ __global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_kernel(GradTable tab,
         }
         return;
     }
+    AdamStep step = {};
+    if (out.adam.state && threadIdx.x == 0) step = adam_begin(out.adam.state, out.adam.lr, out.adam.beta1, out.adam.beta2);
     double v = 0.0;
     for (int i = threadIdx.x; i < before + (int)gridDim.x; i += NVDR_GN_BLOCK) {
         double x = sum;
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(NVDR_GN_BLOCK) grad_norm_kernel(GradTable tab,
         v = gn_join<P>(v, x);
     }
     v = gn_root<P>(gn_block_join<P>(v, lds));
-    if (threadIdx.x == 0) gn_finish(v, out);
+    if (threadIdx.x == 0) gn_finish(v, out, step);
 }
 
 // ---- scaling -------------------------------------------------------------------------------------------------------------------------
@@ -342,7 +351,7 @@ __device__ __forceinline__ void gn_scale_part(char *p, int64_t count, float f)
 template <bool NT, int BLOCK>
 __device__ __forceinline__ void gn_scale_runs(const GradTable &tab, float f)
 {
-    const uint32_t chunks = tab.first[tab.n_tensors], run = tab.run, runs = (chunks - 1) / run + 1;
+    const uint32_t chunks = tab.chunks, run = tab.run, runs = (chunks - 1) / run + 1;
     for (int64_t r = (int64_t)((runs - 1 - blockIdx.x) / gridDim.x) * gridDim.x + blockIdx.x; r >= 0; r -= gridDim.x) {
         const uint32_t c0 = (uint32_t)r * run;
         uint32_t c = min(c0 + run, chunks);
@@ -484,6 +493,8 @@ static unsigned gn_fill(const GradList &l, int64_t *at, int64_t *left, uint64_t 
         ++*at;
     }
     tab.n_tensors = m;
+    tab.chunks = (uint32_t)chunks;
+    for (int q = m; q < 9; ++q) tab.first[q] = (uint32_t)chunks;           // (gn_find compares eight)
     tab.run = 1;
     tab.kept = 0;
     if (chunks == 0) return 0;

@@ -7,7 +7,6 @@ multiplication of the light gradient by 64 (train.py:439-440) enters as a per-te
 device memory, so the launch can be captured in a HIP graph.
 """
 import array
-import contextlib
 import math
 import struct
 
@@ -59,11 +58,6 @@ def _workspace(n, types, clip, device):
     return work.data_ptr(), size, work
 
 
-def _on(device_index):
-    """Makes the device of the call's tensors the current one (launches go to the current device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
-
-
 def grad_norm(tensors, norm_type=2.0, scales=None):
     """The norm of all `tensors` seen as one vector: (sum |scales[k] * g|^p)^(1/p) for norm_type p = 1 or 2, the largest magnitude for
     math.inf; a NaN anywhere gives a NaN.  tensors: a tensor or an iterable of tensors, fp32 / bf16 / fp16 in any mixture and any layout,
@@ -77,11 +71,13 @@ def grad_norm(tensors, norm_type=2.0, scales=None):
     device, data, n, types, _copies = _gradients(tensors, 'grad_norm')
     if device < 0:
         return torch.zeros(())
-    with _on(device):
-        work, size, _owner = _workspace(n, types, 0, device)
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0] if scales else None, len(types), code, math.inf, work, size,
-                                              norm.data_ptr(), None, _lib.stream_ptr()), 'grad_norm')
+    if torch.cuda.current_device() != device:           # (launches go to the current device)
+        with torch.cuda.device(device):
+            return grad_norm(tensors, norm_type, scales)
+    work, size, _owner = _workspace(n, types, 0, device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0] if scales else None, len(types), code, math.inf, work, size,
+                                          norm.data_ptr(), None, _lib.stream_ptr()), 'grad_norm')
     return norm
 
 
@@ -108,18 +104,21 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             if stride <= reach:
                 raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
             reach += (size - 1) * stride
-    with _on(device):
-        work, size, _owner = _workspace(n, types, 1, device)
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        _lib.check(_lib.load().nvdr_grad_clip(data, n, types, len(types), code, max_norm, work, size, norm.data_ptr(), _lib.stream_ptr()), 'clip_grad_norm_')
-        if copies:
-            with torch.no_grad():
-                for g, copy in copies:
-                    g.copy_(copy)
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return clip_grad_norm_(parameters, max_norm, norm_type)
+    work, size, _owner = _workspace(n, types, 1, device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    _lib.check(_lib.load().nvdr_grad_clip(data, n, types, len(types), code, max_norm, work, size, norm.data_ptr(), _lib.stream_ptr()), 'clip_grad_norm_')
+    if copies:
+        with torch.no_grad():
+            for g, copy in copies:
+                g.copy_(copy)
     return norm
 
 
 _ADAM_ROW = struct.Struct('=QQQQqfff4xQqQqfiQii').pack          # nvdr_adam_tensor (_lib.NvdrAdamTensor): filling its fields one by one costs 2 us a tensor
+_UNBOUNDED = (-math.inf, math.inf, 0, 0, 0, 0)
 
 
 class FusedAdam:
@@ -186,7 +185,7 @@ class FusedAdam:
                 raise RuntimeError('FusedAdam.step: parameter %d has no gradient' % i)
         scales = array.array('f', [float(self.grad_scales[i]) * float(grad_mult) for i in live])
         device, data, n, types, _copies = _gradients([self.params[i].grad for i in live], 'FusedAdam')
-        with _on(self.state.get_device()):
+        with torch.cuda.device(self.state.device):
             _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0], len(types), self._norm_code, self.max_norm, self._norm_work.data_ptr() + 16,
                                                   self._norm_work.numel() - 2, self._norm_out.data_ptr(), self._norm_out.data_ptr() + 4, _lib.stream_ptr()), 'grad_norm')
         self._measured = True
@@ -203,9 +202,11 @@ class FusedAdam:
         launch of an iteration but the last, nvdr_adam_step_partial); grad_mult: extra factor on the gradients of this launch (1 / world
         after a summing all-reduce).  With max_norm a launch of all tensors measures the norm first; subsets need measure_norm() before the
         first of them."""
-        idx = range(len(self.params)) if subset is None else list(subset)
-        rows, keep = [], []
-        for i in idx:
+        if torch.cuda.current_device() != self.state.get_device():          # (launches go to the current device)
+            with torch.cuda.device(self.state.device):
+                return self.step(subset, advance, grad_mult)
+        rows, keep, grad_mult = [], [], float(grad_mult)
+        for i in (range(len(self.params)) if subset is None else subset):
             p = self.params[i]
             g = p.grad
             if g is None:
@@ -216,35 +217,31 @@ class FusedAdam:
                     raise RuntimeError('FusedAdam.step: zero_grad needs a contiguous .grad for parameter %d (the persistent scatter-add buffer itself)' % i)
                 g = g.contiguous()
                 keep.append(g)
-            lo, hi, lo_vec, hi_vec = -math.inf, math.inf, None, None
-            c = self.clamps[i]
+            bounds, c = _UNBOUNDED, self.clamps[i]
             if c is not None:
-                lo = -math.inf if c[0] is None else float(c[0])
-                hi = math.inf if c[1] is None else float(c[1])
                 lo_vec = c[2] if len(c) > 2 else None
                 hi_vec = c[3] if len(c) > 3 else None
+                bounds = (-math.inf if c[0] is None else c[0], math.inf if c[1] is None else c[1],
+                          lo_vec.data_ptr() if lo_vec is not None else 0, lo_vec.numel() if lo_vec is not None else 0,
+                          hi_vec.data_ptr() if hi_vec is not None else 0, hi_vec.numel() if hi_vec is not None else 0)
             # lr_scales[i] == 0 freezes the tensor (the C block's lr_scale 0 means "the plain rate": a zero-initialised block trains)
             rate, active = float(self.lr_scales[i]), self.active[i]
             rows.append(_ADAM_ROW(p.data_ptr(), g.data_ptr(), self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr(), p.numel(),
-                                  float(self.grad_scales[i]) * float(grad_mult), lo, hi,
-                                  lo_vec.data_ptr() if lo_vec is not None else 0, lo_vec.numel() if lo_vec is not None else 0,
-                                  hi_vec.data_ptr() if hi_vec is not None else 0, hi_vec.numel() if hi_vec is not None else 0,
-                                  rate or 1.0, bool(self.normalize3[i]), active.data_ptr() if active is not None else 0,
-                                  bool(self.zero_grad_after[i]) and active is not None, rate == 0.0))
+                                  self.grad_scales[i] * grad_mult, *bounds, rate or 1.0, bool(self.normalize3[i]),
+                                  active.data_ptr() if active is not None else 0, bool(self.zero_grad_after[i]) and active is not None, rate == 0.0))
         tab, lib, state = b''.join(rows), _lib.load(), self.state.data_ptr()
         hyper = (self.lr, self.betas[0], self.betas[1], self.eps)
-        with _on(self.state.get_device()):
-            if self.max_norm is not None and subset is None and advance:
-                _lib.check(lib.nvdr_adam_step_clipped(tab, len(rows), *hyper, state, self._norm_code, self.max_norm, self._norm_work.data_ptr(),
-                                                      self._norm_work.numel(), self._norm_out.data_ptr(), _lib.stream_ptr()), 'adam_step')
-                self._measured = False
-                return
-            factor = None
-            if self.max_norm is not None:
-                if subset is None:
-                    self.measure_norm(grad_mult)
-                elif not self._measured:
-                    raise RuntimeError('FusedAdam.step: with max_norm, measure_norm() comes before the first subset of an iteration')
-                factor = self._norm_out.data_ptr() + 4
-                self._measured = not advance
-            _lib.check(lib.nvdr_adam_step_factor(tab, len(rows), *hyper, state, bool(advance), factor, _lib.stream_ptr()), 'adam_step')
+        if self.max_norm is not None and subset is None and advance:
+            _lib.check(lib.nvdr_adam_step_clipped(tab, len(rows), *hyper, state, self._norm_code, self.max_norm, self._norm_work.data_ptr(),
+                                                  self._norm_work.numel(), self._norm_out.data_ptr(), _lib.stream_ptr()), 'adam_step')
+            self._measured = False
+            return
+        factor = None
+        if self.max_norm is not None:
+            if subset is None:
+                self.measure_norm(grad_mult)
+            elif not self._measured:
+                raise RuntimeError('FusedAdam.step: with max_norm, measure_norm() comes before the first subset of an iteration')
+            factor = self._norm_out.data_ptr() + 4
+            self._measured = not advance
+        _lib.check(lib.nvdr_adam_step_factor(tab, len(rows), *hyper, state, bool(advance), factor, _lib.stream_ptr()), 'adam_step')

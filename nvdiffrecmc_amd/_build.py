@@ -33,9 +33,9 @@ SOURCES = [
 
 # -ffp-contract=off: the sampling math must round exactly like the CPU oracle
 # (see include/nvdr_detmath.h); fused operations are written as explicit fmaf.
-# The lists of nvdr_grad_norm / nvdr_grad_clip out of Python tensors: a CPython extension against the installed torch (host code only)
-GRADLIST_SOURCE = os.path.join(CSRC, 'gradlist.cpp')
-GRADLIST = os.path.join(BUILD, '_gradlist.so')
+# nvdr_grad_norm / nvdr_grad_clip for lists of Python tensors: a CPython extension against the installed torch (host code only)
+GRADOPS_SOURCE = os.path.join(CSRC, 'gradops.cpp')
+GRADOPS = os.path.join(BUILD, '_gradops.so')
 
 # -packed-fp32-ops: the compiler makes v_pk_add / mul / fma_f32 from ordinary float code at -O3, and some of their forms have given wrong
 # results now and then on MI355X; the target feature is taken away for every source (the host pass warns that it does not know it).
@@ -94,23 +94,23 @@ def build(force=False, verbose=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError('link failed:\n%s\n%s' % (r.stdout, r.stderr))
-    if force or not os.path.exists(GRADLIST) or os.path.getmtime(GRADLIST) < os.path.getmtime(GRADLIST_SOURCE):
-        _build_gradlist(verbose)
+    if force or not os.path.exists(GRADOPS) or os.path.getmtime(GRADOPS) < max(os.path.getmtime(GRADOPS_SOURCE), hdr_mtime):
+        _build_gradops(verbose)
     return LIB
 
 
-def _build_gradlist(verbose):
+def _build_gradops(verbose):
     import sysconfig
     import torch
     from torch.utils import cpp_extension
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI,
-           '-I' + sysconfig.get_paths()['include']] + ['-I' + d for d in cpp_extension.include_paths()]
-    cmd += [GRADLIST_SOURCE, '-o', GRADLIST] + ['-L' + d for d in cpp_extension.library_paths()] + ['-ltorch_python', '-ltorch_cpu', '-lc10']
+           '-I' + os.path.join(ROOT, 'include'), '-I' + sysconfig.get_paths()['include']] + ['-I' + d for d in cpp_extension.include_paths()]
+    cmd += [GRADOPS_SOURCE, '-o', GRADOPS] + ['-L' + d for d in cpp_extension.library_paths()] + ['-ltorch_python', '-ltorch_cpu', '-lc10']
     if verbose:
         print(' '.join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError('g++ failed for gradlist.cpp:\n%s\n%s' % (r.stdout, r.stderr))
+        raise RuntimeError('g++ failed for gradops.cpp:\n%s\n%s' % (r.stdout, r.stderr))
 
 
 if __name__ == '__main__':

@@ -232,20 +232,23 @@ def load():
     return lib
 
 
-_gradlist = None
+_gradops = None
 
 
-def gradlist():
-    """The extension that reads lists of gradients (csrc/gradlist.cpp).  Raises RuntimeError when it is not built."""
-    global _gradlist
-    if _gradlist is None:
-        path = _build.GRADLIST
+def gradops():
+    """The extension that calls nvdr_grad_norm / nvdr_grad_clip for lists of tensors (csrc/gradops.cpp).  Raises RuntimeError when it is not built."""
+    global _gradops
+    if _gradops is None:
+        path = _build.GRADOPS
         if not os.path.exists(path):
-            raise RuntimeError("_gradlist.so is not built (%s). Build it first: python -c 'import __graft_entry__ as g; g.build()'" % path)
-        spec = importlib.util.spec_from_file_location('_gradlist', path)
-        _gradlist = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_gradlist)
-    return _gradlist
+            raise RuntimeError("_gradops.so is not built (%s). Build it first: python -c 'import __graft_entry__ as g; g.build()'" % path)
+        spec = importlib.util.spec_from_file_location('_gradops', path)
+        ops, lib = importlib.util.module_from_spec(spec), load()
+        spec.loader.exec_module(ops)
+        ops.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in ('nvdr_grad_norm', 'nvdr_grad_clip', 'nvdr_grad_norm_workspace', 'nvdr_last_error')),
+                 getattr(torch._C, '_cuda_getCurrentRawStream', None))
+        _gradops = ops
+    return _gradops
 
 
 def check(rc, what):

@@ -49,7 +49,7 @@
 #define NVDR_GN_ONE_BLOCK 1024          // a short list: one workgroup clips all of it
 #define NVDR_GN_ONE_TENSORS 8
 #define NVDR_GN_ONE_CLIP (64 << 10)     // bytes
-#define NVDR_GN_PATIENCE (1 << 24)      // polls after which a workgroup no longer waits for another (seconds; nothing reaches it)
+#define NVDR_GN_PATIENCE (1 << 28)      // polls after which a workgroup no longer waits for another (minutes; the norm is then a NaN)
 #define NVDR_GN_EPS 1e-6
 
 enum { GN_INF = 0, GN_ONE = 1, GN_TWO = 2 };                // the kernels' norm types
@@ -66,6 +66,7 @@ struct GradTable {
     uint64_t data[NVDR_GN_TENSORS];             // address, the type in the upper two bits
     int64_t n[NVDR_GN_TENSORS];                 // elements, never zero
 };
+static_assert(NVDR_GN_CHUNK == 4 << 10, "gn_fill divides by shifting");
 static_assert(sizeof(GradTable) <= 3900, "the kernel arguments have to fit 4 KB");
 
 typedef uint32_t gn_u4 __attribute__((ext_vector_type(4)));
@@ -431,7 +432,7 @@ static int gn_check(const GradList &l, int norm_type, double max_norm, bool clip
         NVDR_REQUIRE(l.type[k] <= GN_F16, "%s: tensor %lld has type %d", who, (long long)k, (int)l.type[k]);
         NVDR_REQUIRE(l.n[k] >= 0 && l.n[k] < (1ll << 40), "%s: tensor %lld has %lld elements", who, (long long)k, (long long)l.n[k]);
         NVDR_REQUIRE(l.n[k] == 0 || (l.data[k] && (uintptr_t)l.data[k] < (1ull << 62)), "%s: tensor %lld has no memory", who, (long long)k);
-        NVDR_REQUIRE((uintptr_t)l.data[k] % (uintptr_t)gn_size(l.type[k]) == 0, "%s: tensor %lld is not aligned to its elements", who, (long long)k);
+        NVDR_REQUIRE(((uintptr_t)l.data[k] & (uintptr_t)(gn_size(l.type[k]) - 1)) == 0, "%s: tensor %lld is not aligned to its elements", who, (long long)k);
     }
     const int64_t need = gn_workspace(l, clip);
     NVDR_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 7) == 0 && workspace_len >= need), "%s: an 8-byte aligned workspace of %lld doubles is needed, there are %lld",
@@ -480,7 +481,7 @@ static unsigned gn_fill(const GradList &l, int64_t *at, int64_t *left, uint64_t 
         if (n == 0) { ++*at; continue; }
         // directly behind the one before, same type and scale: one tensor
         const bool more = m && tab.data[m - 1] + (uint64_t)(tab.n[m - 1] * size) == word && tab.scale[m - 1] == scale;
-        const uint64_t front = more ? tab.first[m - 1] : chunks, c = front + (uint64_t)(((more ? tab.n[m - 1] : 0) + n + len - 1) / len);
+        const uint64_t front = more ? tab.first[m - 1] : chunks, c = front + (((uint64_t)((more ? tab.n[m - 1] : 0) + n + len - 1)) >> (type == GN_F32 ? 10 : 11));
         if ((!more && m == NVDR_GN_TENSORS) || (m && c >= (1ull << 31))) break;
         if (more) tab.n[m - 1] += n;
         else {

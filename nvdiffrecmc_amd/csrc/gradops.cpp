@@ -1,0 +1,221 @@
+// gradops.cpp -- nvdr_grad_norm and nvdr_grad_clip for lists of Python tensors (optim.py grad_norm, clip_grad_norm_, FusedAdam.measure_norm).
+//
+// The kernels of a short list take 5 us, and a network has hundreds of parameters: asking each gradient for address, length, type, device and
+// layout through Python takes 0.4 us a tensor, and the call around them some 6 us -- more than the work.  Here it is 20 ns a tensor and 2 us a
+// call.  A CPython extension of its own against the installed torch; the C library stays free of torch, and its entries are handed over as
+// addresses (bind), so that there is one copy of it in the process.
+#define PY_SSIZE_T_CLEAN
+#include <torch/csrc/autograd/python_variable.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+#include <vector>
+
+#include "nvdr_hip.h"
+
+static decltype(&nvdr_grad_norm) grad_norm_entry = nullptr;
+static decltype(&nvdr_grad_clip) grad_clip_entry = nullptr;
+static decltype(&nvdr_grad_norm_workspace) workspace_entry = nullptr;
+static decltype(&nvdr_last_error) last_error_entry = nullptr;
+static PyObject *raw_stream = nullptr;              // device index -> handle of its current stream
+
+namespace {
+
+struct Lists {
+    std::vector<void *> data;
+    std::vector<int64_t> n;
+    std::vector<uint8_t> type;
+    std::vector<Py_ssize_t> irregular;              // tensors whose elements do not fill their memory exactly once
+    int device = -1;
+    int64_t count() const { return (int64_t)n.size(); }
+};
+
+// The gradients in `seq`, a list: tensors, or parameters whose gradients are meant (None is left out).  written: the call is going to write to
+// them: their versions go up, as with any operation in place.  false: an exception is set.
+bool collect(PyObject *seq, bool grads, bool written, Lists &l)
+{
+    if (!PyList_Check(seq)) {
+        PyErr_SetString(PyExc_TypeError, "a list is expected");
+        return false;
+    }
+    const size_t most = (size_t)PyList_GET_SIZE(seq);
+    l.data.reserve(most); l.n.reserve(most); l.type.reserve(most);
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
+        PyObject *item = PyList_GET_ITEM(seq, k);
+        if (!THPVariable_Check(item)) {
+            PyErr_Format(PyExc_TypeError, "gradients must be tensors (got %s)", Py_TYPE(item)->tp_name);
+            return false;
+        }
+        const at::Tensor &own = THPVariable_Unpack(item);          // (the list is the caller's own: nobody takes the item out)
+        const at::Tensor &t = grads ? own.grad() : own;
+        if (!t.defined()) continue;
+        int type = -1;
+        switch (t.scalar_type()) {
+        case at::kFloat: type = NVDR_GRAD_F32; break;
+        case at::kBFloat16: type = NVDR_GRAD_BF16; break;
+        case at::kHalf: type = NVDR_GRAD_F16; break;
+        default: break;
+        }
+        if (type < 0) {
+            PyObject *d = PyObject_GetAttrString(item, "dtype");
+            if (d) PyErr_Format(PyExc_ValueError, "gradients must be float32, bfloat16 or float16 (got %S)", d);
+            Py_XDECREF(d);
+            return false;
+        }
+        if (!t.is_cuda() || (l.device >= 0 && t.get_device() != l.device)) {
+            PyErr_SetString(PyExc_RuntimeError, "gradients must reside on one GPU; this path has no CPU fallback");
+            return false;
+        }
+        if (t.layout() != at::kStrided) {
+            PyErr_SetString(PyExc_ValueError, "gradients must be dense");
+            return false;
+        }
+        l.device = (int)t.get_device();
+        if (!t.is_non_overlapping_and_dense()) l.irregular.push_back((Py_ssize_t)l.n.size());
+        l.data.push_back(t.data_ptr());
+        l.n.push_back(t.numel());
+        l.type.push_back((uint8_t)type);
+        if (written && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    return true;
+}
+
+PyObject *irregular_list(const Lists &l)
+{
+    PyObject *r = PyList_New((Py_ssize_t)l.irregular.size());
+    for (size_t i = 0; r && i < l.irregular.size(); ++i) {
+        PyObject *v = PyLong_FromSsize_t(l.irregular[i]);
+        if (!v) { Py_DECREF(r); return nullptr; }
+        PyList_SET_ITEM(r, (Py_ssize_t)i, v);
+    }
+    return r;
+}
+
+bool current_stream(int device, void **stream)
+{
+    PyObject *i = PyLong_FromLong(device), *h = i ? PyObject_CallFunctionObjArgs(raw_stream, i, nullptr) : nullptr;
+    *stream = h ? PyLong_AsVoidPtr(h) : nullptr;
+    Py_XDECREF(i);
+    Py_XDECREF(h);
+    return !PyErr_Occurred();
+}
+
+at::Tensor empty(at::IntArrayRef size, at::ScalarType type, int device)
+{
+    return at::empty(size, at::TensorOptions().dtype(type).device(at::Device(at::kCUDA, (at::DeviceIndex)device)));
+}
+
+PyObject *failed(const char *what, int rc)
+{
+    const char *why = last_error_entry();
+    return PyErr_Format(PyExc_RuntimeError, "%s failed (code %d): %s", what, rc, why ? why : "?");
+}
+
+// no C++ exception passes into the interpreter
+template <class F>
+PyObject *guarded(F f)
+{
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "reading the gradients failed");
+    }
+    return nullptr;
+}
+
+}  // namespace
+
+// norm(tensors, scales, norm_type, max_norm, out, work): a new 0-d tensor, or into `out` (norm, factor) with the workspace `work`; None for no
+// tensors; the positions of irregular ones as a list (then nothing was done).  scales: fp32 bytes or None
+static PyObject *norm(PyObject *, PyObject *args)
+{
+    PyObject *seq, *scales, *out, *work;
+    int code;
+    double max_norm;
+    if (!PyArg_ParseTuple(args, "OOidOO", &seq, &scales, &code, &max_norm, &out, &work)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        Lists l;
+        if (!collect(seq, false, false, l)) return nullptr;
+        if (!l.irregular.empty()) return irregular_list(l);
+        if (out == Py_None && l.device < 0) Py_RETURN_NONE;
+        if (scales != Py_None && (!PyBytes_Check(scales) || PyBytes_GET_SIZE(scales) != 4 * (Py_ssize_t)l.count())) return PyErr_Format(PyExc_ValueError, "a scale for each tensor is expected");
+        at::Tensor result, room;
+        if (out != Py_None) {
+            result = THPVariable_Unpack(out);
+            room = THPVariable_Unpack(work);
+            if (l.device >= 0 && l.device != result.get_device()) return PyErr_Format(PyExc_RuntimeError, "gradients must reside on one GPU; this path has no CPU fallback");
+            l.device = (int)result.get_device();
+        }
+        const c10::DeviceGuard device(at::Device(at::kCUDA, (at::DeviceIndex)l.device));
+        void *stream;
+        if (!current_stream(l.device, &stream)) return nullptr;
+        if (out == Py_None) {
+            result = empty({}, at::kFloat, l.device);
+            room = empty({workspace_entry(l.n.data(), l.type.data(), l.count(), 0)}, at::kDouble, l.device);
+        }
+        float *at = (float *)result.data_ptr();
+        int rc;
+        const float *s = scales == Py_None ? nullptr : (const float *)PyBytes_AS_STRING(scales);
+        Py_BEGIN_ALLOW_THREADS
+        rc = grad_norm_entry(l.data.data(), l.n.data(), l.type.data(), s, l.count(), code, max_norm, (double *)room.data_ptr(), room.numel(), at, out == Py_None ? nullptr : at + 1, stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return failed("grad_norm", rc);
+        return THPVariable_Wrap(result);
+    });
+}
+
+// clip(sequence, grads, norm_type, max_norm): the gradients scaled in place; results as norm's
+static PyObject *clip(PyObject *, PyObject *args)
+{
+    PyObject *seq;
+    int grads, code;
+    double max_norm;
+    if (!PyArg_ParseTuple(args, "Opid", &seq, &grads, &code, &max_norm)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        Lists l;
+        if (!collect(seq, grads != 0, true, l)) return nullptr;
+        if (!l.irregular.empty()) return irregular_list(l);
+        if (l.device < 0) Py_RETURN_NONE;
+        const c10::DeviceGuard device(at::Device(at::kCUDA, (at::DeviceIndex)l.device));
+        void *stream;
+        if (!current_stream(l.device, &stream)) return nullptr;
+        const at::Tensor result = empty({}, at::kFloat, l.device);
+        const int64_t size = workspace_entry(l.n.data(), l.type.data(), l.count(), 1);
+        at::Tensor room;
+        if (size) room = empty({size}, at::kDouble, l.device);
+        float *at = (float *)result.data_ptr();
+        double *w = size ? (double *)room.data_ptr() : nullptr;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = grad_clip_entry(l.data.data(), l.n.data(), l.type.data(), l.count(), code, max_norm, w, size, at, stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return failed("clip_grad_norm_", rc);
+        return THPVariable_Wrap(result);
+    });
+}
+
+// bind(nvdr_grad_norm, nvdr_grad_clip, nvdr_grad_norm_workspace, nvdr_last_error, raw_stream): the library's entries, and where the stream comes from
+static PyObject *bind(PyObject *, PyObject *args)
+{
+    unsigned long long a, b, c, d;
+    PyObject *stream;
+    if (!PyArg_ParseTuple(args, "KKKKO", &a, &b, &c, &d, &stream)) return nullptr;
+    grad_norm_entry = (decltype(grad_norm_entry))(uintptr_t)a;
+    grad_clip_entry = (decltype(grad_clip_entry))(uintptr_t)b;
+    workspace_entry = (decltype(workspace_entry))(uintptr_t)c;
+    last_error_entry = (decltype(last_error_entry))(uintptr_t)d;
+    Py_INCREF(stream);
+    Py_XDECREF(raw_stream);
+    raw_stream = stream;
+    Py_RETURN_NONE;
+}
+
+static PyMethodDef methods[] = {{"norm", norm, METH_VARARGS, "norm(tensors, scales, norm_type, max_norm, out, work)"},
+                                {"clip", clip, METH_VARARGS, "clip(sequence, grads, norm_type, max_norm)"},
+                                {"bind", bind, METH_VARARGS, "bind(nvdr_grad_norm, nvdr_grad_clip, nvdr_grad_norm_workspace, nvdr_last_error, raw_stream)"},
+                                {nullptr, nullptr, 0, nullptr}};
+static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_gradops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+PyMODINIT_FUNC PyInit__gradops(void) { return PyModule_Create(&module); }

@@ -31,31 +31,18 @@ def _max_norm(max_norm):
     return max_norm
 
 
-def _gradients(tensors, what, grads=False, written=False):
-    """The gradients of one call as the library takes them: (device, data, n, types, copies).  Checked there: fp32 / bf16 / fp16 on one GPU.
-    tensors: gradients, or parameters (grads: theirs are meant, None is left out).  One whose elements do not fill their memory exactly once
-    (a slice, an expanded tensor) is replaced by a contiguous copy; copies: the pairs of tensor and copy."""
+def _norm(tensors, scales, code, max_norm, out, work, what):
+    """gradops.norm, with contiguous copies in the place of tensors whose elements do not fill their memory exactly once (a slice, an expanded
+    tensor)."""
     try:
-        device, data, n, types, irregular = _lib.gradlist().collect(tensors, grads, written)
-        if not irregular:
-            return device, data, n, types, ()
-        tensors = [p.grad for p in tensors if p.grad is not None] if grads else list(tensors)
-        copies = [(tensors[i], tensors[i].detach().clone(memory_format=torch.contiguous_format)) for i in irregular]
-        for i, (_, copy) in zip(irregular, copies):
-            tensors[i] = copy
-        device, data, n, types, _ = _lib.gradlist().collect(tensors, False, False)
-        return device, data, n, types, copies
+        r = _lib.gradops().norm(tensors, scales, code, max_norm, out, work)
+        if isinstance(r, list):
+            for i in r:
+                tensors[i] = tensors[i].detach().clone(memory_format=torch.contiguous_format)
+            r = _lib.gradops().norm(tensors, scales, code, max_norm, out, work)
+        return r
     except (TypeError, ValueError) as e:
         raise type(e)('%s: %s' % (what, e)) from None
-
-
-def _workspace(n, types, clip, device):
-    """(address, doubles, owner) of the device memory a call needs, nothing for a short list."""
-    size = _lib.load().nvdr_grad_norm_workspace(n, types, len(types), clip)
-    if size == 0:
-        return None, 0, None
-    work = torch.empty(size, dtype=torch.float64, device=device)
-    return work.data_ptr(), size, work
 
 
 def grad_norm(tensors, norm_type=2.0, scales=None):
@@ -65,20 +52,11 @@ def grad_norm(tensors, norm_type=2.0, scales=None):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
     if scales is not None:
-        scales = array.array('f', scales)
-        if len(scales) != len(tensors):
-            raise ValueError('grad_norm: %d scales for %d tensors' % (len(scales), len(tensors)))
-    device, data, n, types, _copies = _gradients(tensors, 'grad_norm')
-    if device < 0:
-        return torch.zeros(())
-    if torch.cuda.current_device() != device:           # (launches go to the current device)
-        with torch.cuda.device(device):
-            return grad_norm(tensors, norm_type, scales)
-    work, size, _owner = _workspace(n, types, 0, device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0] if scales else None, len(types), code, math.inf, work, size,
-                                          norm.data_ptr(), None, _lib.stream_ptr()), 'grad_norm')
-    return norm
+        scales = array.array('f', scales).tobytes()
+        if len(scales) != 4 * len(tensors):
+            raise ValueError('grad_norm: %d scales for %d tensors' % (len(scales) // 4, len(tensors)))
+    norm = _norm(tensors, scales, code, math.inf, None, None, 'grad_norm')
+    return torch.zeros(()) if norm is None else norm
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -95,26 +73,29 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         norm = grad_norm([p.grad for p in parameters if p.grad is not None], norm_type).item()
         if not math.isfinite(norm):
             raise RuntimeError('clip_grad_norm_: the norm of the gradients is %s' % norm)
-    device, data, n, types, copies = _gradients(parameters, 'clip_grad_norm_', grads=True, written=True)
-    if device < 0:
-        return torch.zeros((), device=parameters[0].device if parameters else None)
-    for g, _ in copies:
-        reach = 0
-        for stride, size in sorted((st, sz) for st, sz in zip(g.stride(), g.shape) if sz != 1):
-            if stride <= reach:
-                raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
-            reach += (size - 1) * stride
-    if torch.cuda.current_device() != device:
-        with torch.cuda.device(device):
-            return clip_grad_norm_(parameters, max_norm, norm_type)
-    work, size, _owner = _workspace(n, types, 1, device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    _lib.check(_lib.load().nvdr_grad_clip(data, n, types, len(types), code, max_norm, work, size, norm.data_ptr(), _lib.stream_ptr()), 'clip_grad_norm_')
-    if copies:
+    try:
+        norm = _lib.gradops().clip(parameters, True, code, max_norm)
+        if not isinstance(norm, list):
+            return torch.zeros((), device=parameters[0].device if parameters else None) if norm is None else norm
+        # gradients whose elements do not lie side by side: through contiguous copies
+        grads = [p.grad for p in parameters if p.grad is not None]
+        originals = [grads[i] for i in norm]
+        for g in originals:
+            reach = 0
+            for stride, size in sorted((st, sz) for st, sz in zip(g.stride(), g.shape) if sz != 1):
+                if stride <= reach:
+                    raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
+                reach += (size - 1) * stride
+        for i in norm:
+            grads[i] = grads[i].detach().clone(memory_format=torch.contiguous_format)
+        copies = [grads[i] for i in norm]
+        norm = _lib.gradops().clip(grads, False, code, max_norm)
         with torch.no_grad():
-            for g, copy in copies:
+            for g, copy in zip(originals, copies):
                 g.copy_(copy)
-    return norm
+        return norm
+    except (TypeError, ValueError) as e:
+        raise type(e)('clip_grad_norm_: %s' % e) from None
 
 
 _ADAM_ROW = struct.Struct('=QQQQqfff4xQqQqfiQii').pack          # nvdr_adam_tensor (_lib.NvdrAdamTensor): filling its fields one by one costs 2 us a tensor
@@ -156,12 +137,11 @@ class FusedAdam:
         self.max_norm, self._norm_code = (None if max_norm is None else _max_norm(max_norm)), _norm_code(norm_type)
         self._measured = False
         dev = self.params[0].device
-        self._norm_out = torch.zeros(2, dtype=torch.float32, device=dev) if max_norm is not None else None       # norm, factor
-        self._norm_view = self._norm_out[0] if max_norm is not None else None
-        self._norm_work = None
-        if max_norm is not None:        # (what the step begins with, and the parts of the norm: enough for any part of the tensors)
-            n, types = array.array('q', [p.numel() for p in self.params]).tobytes(), bytes(len(self.params))
-            self._norm_work = torch.empty(2 + _lib.load().nvdr_grad_norm_workspace(n, types, len(types), 0), dtype=torch.float64, device=dev)
+        self._norm_out = torch.zeros(2, dtype=torch.float32, device=dev)        # norm, factor
+        self._norm_view = self._norm_out[0]
+        # what the step begins with, and the parts of the norm: enough for any part of the tensors
+        n, types = array.array('q', [p.numel() for p in self.params]).tobytes(), bytes(len(self.params))
+        self._norm_work = torch.empty(2 + _lib.load().nvdr_grad_norm_workspace(n, types, len(types), 0), dtype=torch.float64, device=dev)
         self.state = torch.zeros(8, dtype=torch.int32, device=self.params[0].device)     # steps taken, scratch, beta1^t, beta2^t (doubles)
 
     @property
@@ -171,7 +151,7 @@ class FusedAdam:
     @property
     def grad_norm(self):
         """Norm of the gradients of the last step before clipping (0 before the first one; None without max_norm)."""
-        return self._norm_view
+        return None if self.max_norm is None else self._norm_view
 
     def measure_norm(self, grad_mult=1.0):
         """The norm of this iteration's gradients into .grad_norm, and the factor of the updates that follow (max_norm).  step() of all tensors
@@ -183,11 +163,8 @@ class FusedAdam:
         for i in live:
             if self.params[i].grad is None:
                 raise RuntimeError('FusedAdam.step: parameter %d has no gradient' % i)
-        scales = array.array('f', [float(self.grad_scales[i]) * float(grad_mult) for i in live])
-        device, data, n, types, _copies = _gradients([self.params[i].grad for i in live], 'FusedAdam')
-        with torch.cuda.device(self.state.device):
-            _lib.check(_lib.load().nvdr_grad_norm(data, n, types, scales.buffer_info()[0], len(types), self._norm_code, self.max_norm, self._norm_work.data_ptr() + 16,
-                                                  self._norm_work.numel() - 2, self._norm_out.data_ptr(), self._norm_out.data_ptr() + 4, _lib.stream_ptr()), 'grad_norm')
+        scales = array.array('f', [float(self.grad_scales[i]) * float(grad_mult) for i in live]).tobytes()
+        _norm([self.params[i].grad for i in live], scales, self._norm_code, self.max_norm, self._norm_out, self._norm_work[2:], 'FusedAdam')
         self._measured = True
 
     def zero_grad(self, set_to_none=True):

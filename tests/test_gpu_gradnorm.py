@@ -526,6 +526,78 @@ def test_clipped_step_captured(dev):
     assert a.step_count == b.step_count == 5
 
 
+def test_gradients_at_odd_places_update_alike(dev):
+    """Gradients inside a bucket begin anywhere: the same parameters and moments as from gradients of their own, bit for bit, by every path
+    (plain, normal map, sparse with and without zeroing), at lengths that are no multiple of four."""
+    shapes = [(1001, 3), (13, 7, 3), (37, 3), (1,), (2053,), (65, 3)]
+    kw = dict(max_norm=1.0, normalize3=[False, True, True, False, False, False], sparse=[True, False, True, False, False, True], zero_grad=[True, False, False, False, False, True],
+              clamps=[(0.0, 1.0, torch.tensor([0.1, 0.0, 0.2], device=dev)), (-1.0, 1.0), None, (None, 0.7), (0.01, None), (None, None, None, torch.tensor([0.5, 0.6], device=dev))])
+    a, b = _adam(shapes, dev, 7, **kw), _adam(shapes, dev, 7, **kw)
+    buf = torch.full((20000,), 9.0, device=dev)
+    for t in range(3):
+        h = _grads(shapes, t)
+        h[0][64:128] = 0.0                                                  # a tile without a gradient
+        at = 3
+        for x, y, g in zip(a.params, b.params, h):
+            x.grad = g.to(dev)
+            y.grad = buf[at:at + g.numel()].view(g.shape)
+            y.grad.copy_(g)
+            at += g.numel() + 1
+        a.step()
+        b.step()
+        assert a.grad_norm.item() == b.grad_norm.item()
+        for i in range(len(shapes)):
+            assert torch.equal(a.params[i], b.params[i]) and torch.equal(a.exp_avg[i], b.exp_avg[i]) and torch.equal(a.exp_avg_sq[i], b.exp_avg_sq[i]), (t, i)
+            assert torch.equal(a.params[i].grad, b.params[i].grad), (t, i)
+            assert bool((b.params[i].grad == 0).all()) == kw['zero_grad'][i], (t, i)
+            if a.active[i] is not None:
+                assert torch.equal(a.active[i], b.active[i])
+    gaps = torch.ones(20000, dtype=torch.bool)
+    at = 3
+    for s in shapes:
+        gaps[at:at + math.prod(s)] = False
+        at += math.prod(s) + 1
+    assert bool((buf.cpu()[gaps] == 9.0).all())
+
+
+def test_a_frozen_sparse_texture_only_loses_its_gradient(dev):
+    opt = _adam([(40, 40, 3), (8, 3)], dev, 8, max_norm=1.0, sparse=[True, False], zero_grad=[True, False], lr_scales=[0.0, 1.0])
+    h = _grads([(40, 40, 3), (8, 3)], 1)
+    before = opt.params[0].detach().clone()
+    for q, g in zip(opt.params, h):
+        q.grad = g.to(dev)
+    opt.step()
+    close(opt.grad_norm.item(), norm64(h[1:], 2.0), NORM_TOL)
+    assert torch.equal(opt.params[0], before) and bool((opt.params[0].grad == 0).all())
+    assert bool((opt.exp_avg[0] == 0).all()) and bool((opt.active[0] == 0).all())
+
+
+def test_a_step_longer_than_the_cache_is_the_same_step(dev):
+    """7 M parameters at once (moments past the caches) and tensor by tensor (not): the same bits."""
+    shapes = [(1201, 1203, 3), (1000, 1001, 3), (257, 3), (31, 33, 3)]
+    kw = dict(max_norm=0.5, normalize3=[False, True, False, True], clamps=[(0.0, 1.0), (-1.0, 1.0), None, None])
+    a, b = _adam(shapes, dev, 9, **kw), _adam(shapes, dev, 9, **kw)
+    assert 28 * sum(p.numel() for p in a.params) > 160 << 20 > 28 * max(p.numel() for p in a.params)
+    for t in range(2):
+        for x, y, g in zip(a.params, b.params, _grads(shapes, t)):
+            x.grad, y.grad = g.to(dev), g.to(dev)
+        a.step()
+        b.measure_norm()
+        for i in range(4):
+            b.step(subset=[i], advance=(i == 3))
+        for i in range(4):
+            assert torch.equal(a.params[i], b.params[i]) and torch.equal(a.exp_avg[i], b.exp_avg[i]) and torch.equal(a.exp_avg_sq[i], b.exp_avg_sq[i]), (t, i)
+
+
+def test_a_threshold_given_later(dev):
+    a, b = _adam(SHAPES, dev, 10, **SETUP), _adam(SHAPES, dev, 10, max_norm=0.5, **SETUP)
+    a.max_norm = 0.5
+    for x, y, g in zip(a.params, b.params, _grads(SHAPES, 1)):
+        x.grad, y.grad = g.to(dev), g.to(dev)
+    a.step(); b.step()
+    assert all(torch.equal(x, y) for x, y in zip(a.params, b.params)) and a.grad_norm.item() == b.grad_norm.item() > 0.5
+
+
 # ---- together, as the iteration uses them -------------------------------------------------------------------------------------------------
 
 def test_iteration_with_clipping_fused_and_composed_agree(dev):

@@ -108,8 +108,8 @@ def test_workspace_of_a_list():
 
 def test_a_missing_extension_is_an_error(monkeypatch):
     from nvdiffrecmc_amd import _build
-    monkeypatch.setattr(_lib, '_gradlist', None)
-    monkeypatch.setattr(_build, 'GRADLIST', '/nonexistent/_gradlist.so')
+    monkeypatch.setattr(_lib, '_gradops', None)
+    monkeypatch.setattr(_build, 'GRADOPS', '/nonexistent/_gradops.so')
     with pytest.raises(RuntimeError, match='not built'):
         optim.grad_norm([torch.zeros(3)])
 

@@ -22,11 +22,14 @@
 //   norm   one contiguous run per workgroup, plain loads          515 | 104 | 12.4
 //          the same with non-temporal loads                       458 |  92 | 12.5
 //          runs of 128 KB dealt in turn, non-temporal             449 |  96 | 12.4      (7.0 TB/s; 32 KB runs: 468 | 132 | 13.2)
+//          finished by its own first workgroup, not by a kernel   447 |  95 | 10.8
 //   clip   one contiguous run per workgroup, plain               1783 | 357 | 23.4
 //          the last 160 MB of the norm's pass loaded to stay,
 //          the scaling from the end to the front, non-temporal   1675 | 307 | 23.4
 //          runs of 128 KB dealt in turn                          1581 | 300 | 23.3
 //          scaling by 256 workgroups of 1024, eight loads deep   1472 | 293 | 24.7      (6.2 TB/s of reading and writing)
+// The time of a short list is that of its launches: 0.8 MB take 5.8 us on the device and 6.4 a call, clipped 4.3 + 4.6 and 10.9; one workgroup
+// clips 64 KB in one launch, 6.8 us where the two launches take 8.6 (at 128 KB 8.5 against 8.7, and 8.1 against 6.7 in a captured graph).
 // A list that fits the last-level cache is left there: plain loads and stores (non-temporal ones cost 29 instead of 23 us at 43 MB), for the
 // scaling and for whoever reads the gradients next.
 #include <stdlib.h>

@@ -372,7 +372,8 @@ __device__ __forceinline__ void gn_scale_runs(const GradTable &tab, float f)
     }
 }
 
-// n_part > 0: every workgroup adds the parts up itself, in the same order, and the first one writes the norm; n_part = 0: the factor is there.  NT: the list is longer than what stays in the cache.
+// n_part > 0: every workgroup adds the parts up itself, in the same order, and the first one writes the norm; n_part = 0: the factor is there.
+// NT: the list is longer than what stays in the cache.
 template <int P, bool NT>
 __global__ void __launch_bounds__(NT ? NVDR_GN_STREAM_BLOCK : NVDR_GN_BLOCK)
 grad_scale_kernel(GradTable tab, const double *__restrict__ part, int n_part, double max_norm, float *__restrict__ norm, const float *__restrict__ factor)
@@ -522,7 +523,7 @@ extern "C" int64_t nvdr_grad_norm_workspace(const int64_t *n, const uint8_t *typ
 #define NVDR_GN_STARTS 64
 struct GradLaunches {
     int64_t start[NVDR_GN_STARTS], left[NVDR_GN_STARTS];        // of the first launches: the scaling takes them in reverse
-    int64_t count = 0, end = 0;
+    int64_t count = 0;
     int n_part = 0;
 };
 

@@ -261,6 +261,8 @@ static int adam_table(const nvdr_adam_tensor *tensors, int n_tensors, double lr,
     for (int k = 0; k < n_tensors; ++k) {
         const nvdr_adam_tensor &t = tensors[k];
         NVDR_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq && t.n >= 0, "adam_step: tensor %d has a NULL buffer", k);
+        for (int j = 0; j < k; ++j)
+            NVDR_REQUIRE(tensors[j].param != t.param || !t.n || !tensors[j].n, "adam_step: tensors %d and %d are the same (two workgroups would update it)", j, k);
         NVDR_REQUIRE(!t.lo_vec || t.lo_vec_n > 0, "adam_step: tensor %d: lo_vec without length", k);
         NVDR_REQUIRE(!t.hi_vec || t.hi_vec_n > 0, "adam_step: tensor %d: hi_vec without length", k);
         NVDR_REQUIRE(!t.normalize3 || t.n % 3 == 0, "adam_step: tensor %d: normalize3 needs a multiple of three elements", k);

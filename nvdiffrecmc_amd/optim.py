@@ -48,7 +48,8 @@ def _norm(tensors, scales, code, max_norm, out, work, what):
 def grad_norm(tensors, norm_type=2.0, scales=None):
     """The norm of all `tensors` seen as one vector: (sum |scales[k] * g|^p)^(1/p) for norm_type p = 1 or 2, the largest magnitude for
     math.inf; a NaN anywhere gives a NaN.  tensors: a tensor or an iterable of tensors, fp32 / bf16 / fp16 in any mixture and any layout,
-    on one GPU.  Returns a 0-d fp32 tensor on that GPU (0 on the CPU for an empty list); nothing waits for it.  Sums are kept in fp64."""
+    on one GPU.  Returns a 0-d fp32 tensor on that GPU (0 on the CPU for an empty list); nothing waits for it, and no gradient flows through it.
+    Sums are kept in fp64."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
     if scales is not None:
@@ -188,6 +189,8 @@ class FusedAdam:
             g = p.grad
             if g is None:
                 raise RuntimeError('FusedAdam.step: parameter %d has no gradient' % i)
+            if g.dtype is not torch.float32:
+                raise RuntimeError('FusedAdam.step: the gradient of parameter %d must be float32 (got %s)' % (i, g.dtype))
             if not g.is_contiguous():
                 if self.zero_grad_after[i]:
                     # a copy would be zeroed instead of the buffer the producer scatter-adds into
@@ -220,5 +223,5 @@ class FusedAdam:
             elif not self._measured:
                 raise RuntimeError('FusedAdam.step: with max_norm, measure_norm() comes before the first subset of an iteration')
             factor = self._norm_out.data_ptr() + 4
-            self._measured = not advance
         _lib.check(lib.nvdr_adam_step_factor(tab, len(rows), *hyper, state, bool(advance), factor, _lib.stream_ptr()), 'adam_step')
+        self._measured = self._measured and not advance

@@ -263,6 +263,28 @@ def test_on_another_stream(dev):
     assert_scaled(g, h, factor64(2.0 * want, 1.0))
 
 
+def test_many_norms_at_once_on_several_streams(dev):
+    """Norms that overlap on the device: each waits for its own workgroups only and has a workspace of its own."""
+    from nvdiffrecmc_amd.optim import clip_grad_norm_, grad_norm
+    sizes = [(5000001, F32), (70001, BF16), (1200007, F16), (333, F32)]
+    host = [[values(n, 50 * k + i, t) for i, (n, t) in enumerate(sizes)] for k in range(4)]
+    want = [norm64(h, 2.0) for h in host]
+    grads = [[x.to(dev) for x in h] for h in host]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = [[] for _ in range(4)]
+    for _ in range(30):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(grad_norm(grads[k]))
+                got[k].append(clip_grad_norm_(params_of(grads[k]), 2.0 * want[k]))        # (nothing to scale)
+    torch.cuda.synchronize()
+    for k in range(4):
+        first = got[k][0].item()
+        close(first, want[k], NORM_TOL, k)
+        assert all(x.item() == first for x in got[k]), k
+
+
 def test_two_captured_graphs_replayed_in_turn(dev):
     """Each graph owns its workspace; every replay sees the gradients of its moment, with eager calls in between."""
     from nvdiffrecmc_amd.optim import clip_grad_norm_, grad_norm
@@ -587,6 +609,29 @@ def test_a_step_longer_than_the_cache_is_the_same_step(dev):
             b.step(subset=[i], advance=(i == 3))
         for i in range(4):
             assert torch.equal(a.params[i], b.params[i]) and torch.equal(a.exp_avg[i], b.exp_avg[i]) and torch.equal(a.exp_avg_sq[i], b.exp_avg_sq[i]), (t, i)
+
+
+def test_the_same_tensor_twice_is_refused(dev):
+    from nvdiffrecmc_amd.optim import FusedAdam
+    opt = _adam(SHAPES, dev, 11, max_norm=1.0, **SETUP)
+    for q, g in zip(opt.params, _grads(SHAPES, 1)):
+        q.grad = g.to(dev)
+    opt.measure_norm()
+    with pytest.raises(RuntimeError, match='the same'):
+        opt.step(subset=[1, 0, 1])
+    opt.step(subset=[0, 1], advance=False)                                  # (a refused launch leaves the measured norm)
+    if hasattr(opt.params[2], 'grad_dtype'):
+        opt.params[2].grad = None
+        opt.params[2].grad_dtype = BF16
+        opt.params[2].grad = torch.ones(SHAPES[2], dtype=BF16, device=dev)
+        with pytest.raises(RuntimeError, match='float32'):
+            opt.step(subset=[2, 3])
+    p = torch.nn.Parameter(torch.ones(5, device=dev))
+    p.grad = torch.ones(5, device=dev)
+    for kw in ({}, {'max_norm': 1.0}):
+        with pytest.raises(RuntimeError, match='the same'):
+            FusedAdam([p, p], **kw).step()
+    assert bool((p == 1).all())
 
 
 def test_a_threshold_given_later(dev):

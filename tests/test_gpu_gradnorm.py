@@ -680,3 +680,65 @@ def test_several_rank_schedule_with_clipping_follows_the_plain_one(geometry, gra
     b.finish()
     assert (a._graphs is not None) == graph and (b._graphs is not None) == graph
     assert a.opt.step_count == b.opt.step_count == 8
+
+
+_TWO_RANKS = r'''
+import json, os, sys, torch, torch.distributed as dist
+sys.path.insert(0, %r)
+from nvdiffrecmc_amd.trainer import DirectLightingStep
+rank, world = int(os.environ['RANK']), int(os.environ['WORLD_SIZE'])
+torch.cuda.set_device(0)
+if world > 1:
+    dist.init_process_group('gloo', rank=rank, world_size=world)
+per = 4 // world
+mine = list(range(rank * per, (rank + 1) * per))
+st = DirectLightingStep('bob', 96, 4, view=mine, n_views=4, device='cuda:0', lr=0.03, tex_res=512, pixel_index_offset=mine[0] * 96 * 96,
+                        use_graph=os.environ['USE_GRAPH'] == '1', exchange_mode=os.environ['EXCHANGE'], max_grad_norm=0.002)
+losses, norms = [], []
+for it in range(8):
+    losses.append(float(st.step(world).detach()))
+    norms.append(st.opt.grad_norm.item())
+st.finish()
+out = {'rank': rank, 'losses': losses, 'norms': norms, 'steps': st.opt.step_count, 'sums': [float(p.detach().double().sum()) for p in st.params]}
+print('RESULT ' + json.dumps(out), flush=True)
+if world > 1:
+    dist.barrier()
+    dist.destroy_process_group()
+'''
+
+
+@pytest.mark.parametrize('graph,exchange', [('0', 'dense'), ('1', 'dense'), ('1', 'sparse')], ids=['eager', 'hip_graphs', 'hip_graphs_sparse'])
+def test_two_ranks_clip_by_the_norm_of_the_batch(graph, exchange, dev):
+    """Four views on two ranks: the norm is that of the averaged gradients, the same on both, and the run follows the one-rank run (to the
+    tolerances of the test of the unclipped schedule; the norm, a sum of squares of such gradients, to 1e-2)."""
+    import json
+    import os
+    import socket
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+    def run(world, rank, port):
+        env = dict(os.environ, MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), USE_GRAPH=graph, EXCHANGE=exchange)
+        return subprocess.Popen([sys.executable, '-c', _TWO_RANKS % root], env=env, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, cwd=root)
+
+    def result(p):
+        out, err = p.communicate(timeout=100)
+        assert p.returncode == 0, out[-2000:] + err[-3000:]
+        return json.loads([line for line in out.splitlines() if line.startswith('RESULT ')][-1][7:])
+
+    def port():
+        with socket.socket() as s:
+            s.bind(('127.0.0.1', 0))
+            return s.getsockname()[1]
+    one = result(run(1, 0, port()))
+    at = port()
+    two = sorted((result(p) for p in [run(2, r, at) for r in range(2)]), key=lambda d: d['rank'])
+    assert one['steps'] == two[0]['steps'] == two[1]['steps'] == 8
+    assert two[0]['norms'] == two[1]['norms']
+    for it in range(8):
+        pair = 0.5 * (two[0]['losses'][it] + two[1]['losses'][it])
+        assert abs(pair - one['losses'][it]) <= 2e-4 * abs(one['losses'][it]), (it, pair, one['losses'][it])
+        assert one['norms'][it] > 0.002 and abs(two[0]['norms'][it] - one['norms'][it]) <= 1e-2 * one['norms'][it], (it, two[0]['norms'][it], one['norms'][it])
+    for a, b, c in zip(two[0]['sums'], two[1]['sums'], one['sums']):
+        assert abs(a - b) <= 1e-9 * abs(a) and abs(a - c) <= 1e-4 * abs(c)

@@ -22,14 +22,14 @@
 //   norm   one contiguous run per workgroup, plain loads          515 | 104 | 12.4
 //          the same with non-temporal loads                       458 |  92 | 12.5
 //          runs of 128 KB dealt in turn, non-temporal             449 |  96 | 12.4      (7.0 TB/s; 32 KB runs: 468 | 132 | 13.2)
-//          finished by its own first workgroup, not by a kernel   447 |  95 | 10.8
+//          finished by its own first workgroup, not by a kernel   447 |  95 | 10.8      (wavefronts joined by DPP: 10.4)
 //   clip   one contiguous run per workgroup, plain               1783 | 357 | 23.4
 //          the last 160 MB of the norm's pass loaded to stay,
 //          the scaling from the end to the front, non-temporal   1675 | 307 | 23.4
 //          runs of 128 KB dealt in turn                          1581 | 300 | 23.3
 //          scaling by 256 workgroups of 1024, eight loads deep   1472 | 293 | 24.7      (6.2 TB/s of reading and writing)
-// The time of a short list is that of its launches: 0.8 MB take 5.8 us on the device and 6.4 a call, clipped 4.3 + 4.6 and 10.9; one workgroup
-// clips 64 KB in one launch, 6.8 us where the two launches take 8.6 (at 128 KB 8.5 against 8.7, and 8.1 against 6.7 in a captured graph).
+// The time of a short list is that of its launches: 0.8 MB take 5.4 us on the device and 6.6 a call, clipped 4.1 + 4.2 and 10.0; one workgroup
+// clips 64 KB in one launch, 6.8 us where the two launches took 8.6 (at 128 KB 8.5 against 8.7, and 8.1 against 6.7 in a captured graph).
 // A list that fits the last-level cache is left there: plain loads and stores (non-temporal ones cost 29 instead of 23 us at 43 MB), for the
 // scaling and for whoever reads the gradients next.
 #include <stdlib.h>
@@ -109,14 +109,29 @@ __device__ __forceinline__ double gn_join(double a, double b)
     return a + b;
 }
 
-// the sum over the workgroup, in every thread; `lds`: one double per wavefront
+// v joined with the value of the lane that the DPP control names (lanes it names none for: with zero, which changes no sum and no maximum)
+template <int P, int CTRL, int ROWS>
+__device__ __forceinline__ double gn_dpp(double v)
+{
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, ROWS, 0xf, false);
+    return gn_join<P>(v, __longlong_as_double((long long)((unsigned long long)hi << 32 | lo)));
+}
+
+// the sum over the workgroup, in every thread; `lds`: one double per wavefront.  Within a wavefront by DPP (rows of sixteen lanes, then row to
+// row into the last lane): 0.4 us less a kernel than six exchanges through the LDS hardware.
 template <int P>
 __device__ __forceinline__ double gn_block_join(double v, double *lds)
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = gn_join<P>(v, __shfl_xor(v, o));
+    v = gn_dpp<P, 0x111, 0xf>(v);          // row_shr:1
+    v = gn_dpp<P, 0x112, 0xf>(v);          // row_shr:2
+    v = gn_dpp<P, 0x114, 0xf>(v);          // row_shr:4
+    v = gn_dpp<P, 0x118, 0xf>(v);          // row_shr:8
+    v = gn_dpp<P, 0x142, 0xa>(v);          // row_bcast:15 into rows 1 and 3
+    v = gn_dpp<P, 0x143, 0xc>(v);          // row_bcast:31 into rows 2 and 3
     __syncthreads();                                        // (a second call: the first one's values have been read)
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = lds[0];
     for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = gn_join<P>(v, lds[w]);

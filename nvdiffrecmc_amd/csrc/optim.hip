@@ -15,7 +15,7 @@
 //
 // Bytes bound it: 28 per parameter.  10.7 M parameters of the scene's set, 298 MB: 72 us with one element a lane and access, 64 us with
 // sixteen bytes, 48 us (6.2 TB/s, what a large copy reaches) with the moments past the caches.  Textures by tiles (12 bytes a texel where
-// nothing is to do): 3 x 1024^2 at a quarter of the tiles 23.7 -> 18.8 us, at a twentieth 15.0 -> 12.5 us.
+// nothing is to do): 3 x 1024^2 at a quarter of the tiles 23.7 -> 19 us, at a twentieth 15.0 -> 12.5 us.
 #include "common.h"
 #include "gradnorm.h"
 #include "nvdr_hip.h"

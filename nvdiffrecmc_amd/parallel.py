@@ -273,8 +273,8 @@ class GradientExchange:
         b = self.buckets[k]
         cuda = b.is_cuda
         if cuda and self._side is None:
-            # (normal priority, as in round 5: a HIGH-priority side stream here -- tried in round 6 to keep it off the main stream's hardware queue --
-            # went with a sporadic stall of the tile-sparse schedule, one run in three; the dense exchange has no side stream at all)
+            # (the default priority: with a side stream of another one the tile-sparse schedule stalled, one run in three; the dense exchange has no
+            # side stream at all)
             self._side = torch.cuda.Stream(device=b.device)
         if cuda:
             self._side.wait_event(self._ev_start)        # the main stream as of start(), not as of now

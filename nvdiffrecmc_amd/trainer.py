@@ -51,7 +51,7 @@ def _capture_graph(g, **kw):
     """torch.cuda.graph(g, ...) with THREAD-LOCAL capture errors.  The default ('global') makes every "unsafe" HIP call of ANY thread an error while a
     stream captures -- and the process group's watchdog thread polls its pending collectives with hipEventQuery: a capture that begins while a
     collective of the warm-up iterations is still on the watchdog's list died, once in ~25 runs of the several-rank schedule, with "operation not
-    permitted when stream is capturing" (round 6, sessions 29-31; `tools/capture_mode_probe.py` shows it deterministically).  Thread-local mode keeps
+    permitted when stream is capturing".  Thread-local mode keeps
     the check for the capturing thread, which is the one whose calls end up in the graph."""
     return torch.cuda.graph(g, capture_error_mode='thread_local', **kw)
 
@@ -874,7 +874,7 @@ class DirectLightingStep:
             if getattr(self, '_build_side', None) is None:
                 # The DEFAULT priority: work on streams of different priorities has hung on this runtime for good.  HIP deals its streams
                 # to four hardware queues, so one in four late streams shares the main stream's queue and the rebuild then runs in line
-                # with it (tools/side_graph_probe.py) -- slower, the same results.
+                # with it -- slower, the same results.
                 self._build_side = torch.cuda.Stream(device=self.dev)
                 self._ev_build, self._ev_main = torch.cuda.Event(), torch.cuda.Event()
             with _capture_graph(g1):

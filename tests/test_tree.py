@@ -1,0 +1,34 @@
+"""What holds for the files of the tree as a whole."""
+import ast
+import glob
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+DIRS = ('nvdiffrecmc_amd', 'tools', 'tests', 'oracle', 'perf')
+
+
+def _files(*suffixes):
+    out = [f for d in DIRS for f in glob.glob(os.path.join(ROOT, d, '**', '*'), recursive=True) if f.endswith(suffixes)]
+    return out + [f for f in glob.glob(os.path.join(ROOT, '*')) if f.endswith(suffixes)]
+
+
+def test_every_stream_has_the_default_priority():
+    """Work on streams of different priorities has hung on this runtime for good."""
+    found = []
+    for f in _files('.py'):
+        for node in ast.walk(ast.parse(open(f).read())):
+            if isinstance(node, ast.Call):
+                found += [(f, node.lineno, k.arg) for k in node.keywords if k.arg in ('priority', 'is_high_priority_stream')]
+    for f in _files('.hip', '.cpp', '.h', '.c'):
+        if re.search(r'hip(StreamCreate|ExtStreamCreate)With(Priority|CUMask)', open(f).read()):
+            found.append(f)
+    assert not found
+
+
+def test_tools_that_are_named_exist():
+    """The documents and the sources point to no tool that is gone."""
+    files = [os.path.join(ROOT, f) for f in ('README.md', 'DESIGN.md', 'INTEGRATION.md')] + _files('.py', '.hip', '.cpp', '.h')
+    named = {(os.path.relpath(f, ROOT), m) for f in files for m in re.findall(r'\btools/[\w/]+\.(?:py|sh|hip|c|txt)\b', open(f).read())}
+    assert len(named) > 20
+    assert not sorted((f, m) for f, m in named if not os.path.exists(os.path.join(ROOT, m)))

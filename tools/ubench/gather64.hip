@@ -6,7 +6,7 @@
 //   single  one record per lane and step                                   -> known: records x 64 B requested
 //   pair    records 2j and 2j + 1 (the two halves of ONE 128-byte line), the second after the first has arrived
 //           -> if an L2 miss fills 128 B, the second half hits L2: TCC_MISS ~ records / 2
-// Run under rocprofv3 (tools/sessions/r04_s29.sh): one pass with --pmc FETCH_SIZE, one with --pmc TCC_REQ_sum TCC_MISS_sum; the
+// Run under rocprofv3: one pass with --pmc FETCH_SIZE, one with --pmc TCC_REQ_sum TCC_MISS_sum; the
 // kernel names carry the pattern and the array size.  Printed here: records fetched and the time of each launch.
 // build: hipcc --offload-arch=gfx950 -O3 gather64.hip -o gather64 ; run: ./gather64
 #include <hip/hip_runtime.h>

@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, do
         // its update is p - step * 0 / (0 + eps) = p, a clamp of a value the first step already clamped.  Tiles with an all-zero
         // gradient and no history are therefore skipped after reading the gradient alone: 12 instead of 84 bytes per texel, EXACTLY
         // the same parameters (step 1 visits every tile, so that the clamps / the normalisation have been applied to whatever the
-        // initial values were).  `active[tile]` remembers history.  zero_grad: the gradient of a visited tile is zeroed behind the
+        // initial values were; a step whose factor is a NaN or infinite makes 0 * factor a NaN, as in a dense tensor, and visits every tile
+        // too; a normal is not normalised again where nothing else is done, a rounding or two of it).  `active[tile]` remembers history.  zero_grad: the gradient of a visited tile is zeroed behind the
         // update, so that a scatter-add backward (nvdr_texture_lookup_bwd into a persistent buffer) needs no memset of 3 x 12.6 MB per
         // iteration.
         //
@@ -197,9 +198,10 @@ __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, do
 #pragma unroll
             for (int j = 0; j < ADAM_TILES; ++j)
                 any |= (__ballot(g[j][0] != 0.0f || g[j][1] != 0.0f || g[j][2] != 0.0f) != 0ull ? 1u : 0u) << j;      // (a NaN compares unequal to zero)
+            const bool spoiled = !(T.grad_scale * S.factor * 0.0f == 0.0f);
             if (T.frozen) visit = 0;
-            else if (S.step > 1) visit = any | history;
-            if (!T.frozen && mine && ((any & ~history) >> lane & 1u)) T.active[tile0 + lane] = 1;
+            else if (S.step > 1 && !spoiled) visit = any | history;
+            if (!T.frozen && mine && (((spoiled ? visit : any) & ~history) >> lane & 1u)) T.active[tile0 + lane] = 1;
         }
 #pragma unroll 1
         for (int j = 0; j < ADAM_TILES; ++j) {

@@ -85,7 +85,7 @@ __device__ __forceinline__ void adam_store(const float (&x)[3], float *p)
 }
 
 struct AdamConst {
-    float factor, step_size, bc2_sqrt, beta2, omb1, omb2, eps;
+    float scale, step_size, bc2_sqrt, beta2, omb1, omb2, eps;
 };
 
 // the moments and the parameter of N elements from e on
@@ -107,7 +107,7 @@ __device__ __forceinline__ void adam_update(const nvdr_adam_tensor &T, const Ada
     }
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-        const float gg = g[c] * T.grad_scale * k.factor;
+        const float gg = g[c] * k.scale;
         m[c] = m[c] + (gg - m[c]) * k.omb1;                         // lerp_(grad, 1 - beta1)
         v[c] = v[c] * k.beta2 + (k.omb2 * gg) * gg;                 // mul_(beta2).addcmul_(grad, grad, value = 1 - beta2)
         const float denom = sqrtf(v[c]) / k.bc2_sqrt + k.eps;
@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, do
     // the hyper-parameters arrive as doubles, like the Python floats torch's Adam computes 1 - beta from: (float)(1 - 0.999) is
     // 0.001f, 1 - 0.999f is 1.3e-5 off (visible in the parameters after ten steps)
     // lr_scale: this tensor's learning rate (train.py:336-338: position / material / light; a zero-initialised block: the plain rate)
-    const AdamConst c = {S.factor, S.step_size * (T.lr_scale == 0.0f ? 1.0f : T.lr_scale), S.bc2_sqrt, (float)beta2d, (float)(1.0 - beta1d), (float)(1.0 - beta2d), eps};
+    // grad_scale and the factor as one product: an outlier times the scale alone may be infinite where clipping bounds it
+    const AdamConst c = {T.grad_scale * S.factor, S.step_size * (T.lr_scale == 0.0f ? 1.0f : T.lr_scale), S.bc2_sqrt, (float)beta2d, (float)(1.0 - beta1d), (float)(1.0 - beta2d), eps};
     const bool wide_g = ((uintptr_t)T.grad & 15) == 0, wide_m = ((uintptr_t)T.exp_avg & 15) == 0, wide_v = ((uintptr_t)T.exp_avg_sq & 15) == 0,
                wide_p = ((uintptr_t)T.param & 15) == 0;
     if (T.frozen && !(T.active && T.zero_grad)) return;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, do
 #pragma unroll
             for (int j = 0; j < ADAM_TILES; ++j)
                 any |= (__ballot(g[j][0] != 0.0f || g[j][1] != 0.0f || g[j][2] != 0.0f) != 0ull ? 1u : 0u) << j;      // (a NaN compares unequal to zero)
-            const bool spoiled = !(T.grad_scale * S.factor * 0.0f == 0.0f);
+            const bool spoiled = !(c.scale * 0.0f == 0.0f);
             if (T.frozen) visit = 0;
             else if (S.step > 1 && !spoiled) visit = any | history;
             if (!T.frozen && mine && (((spoiled ? visit : any) & ~history) >> lane & 1u)) T.active[tile0 + lane] = 1;

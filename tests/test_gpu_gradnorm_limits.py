@@ -63,3 +63,51 @@ def test_tiles_follow_the_dense_step_where_the_norm_is_not_finite(subsets, when,
                 assert bool(b.params[i].isnan().all()) and (b.active[i] is None or bool((b.active[i] != 0).all())), (t, i)
             elif i < 2:
                 assert not bool(b.params[i].isnan().any()), (t, i)
+
+
+# ---- an outlier that only clipping keeps in range ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('kind', ['plain', 'normal map', 'tiles'])
+@pytest.mark.parametrize('subsets', [False, True], ids=['whole', 'subsets'])
+def test_an_outlier_beyond_fp32_behind_its_scale_is_clipped(subsets, kind, dev):
+    """1e37 * 64 is over fp32's range, its clipped value is max_norm.  The factor, 10 / 6.4e38 = 1.6e-38, is a normal number: rounded once, the
+    product with 64 exact, the product with the gradient rounded once: 2^-23 relative; the first moment (0.1 rounded, one product) 2^-23
+    more, the second (0.001 rounded, two products, the gradient's error twice) 6 * 2^-24 more, each 2^-21 at most."""
+    shape = (20, 16, 3)
+    g = _values(shape, 1).view(-1)
+    g[7], g[300] = 1e37, -3e36
+    g = g.view(shape)
+    opt = _adam([torch.full(shape, 0.5), torch.full((9,), 0.5)], dev, max_norm=10.0, grad_scales=[64.0, 1.0], sparse=[kind == 'tiles', False], normalize3=[kind == 'normal map', False])
+    h = [g, torch.full((9,), 2.0)]
+    for q, x in zip(opt.params, h):
+        q.grad = x.to(dev)
+    if subsets:
+        opt.measure_norm()
+        opt.step(subset=[0], advance=False)
+        opt.step(subset=[1])
+    else:
+        opt.step()
+    eff = [h[0].double() * 64.0, h[1].double()]
+    norm = math.sqrt(sum(float((x * x).sum()) for x in eff))
+    assert math.isinf(opt.grad_norm.item()) and 2.0 ** -126 < 10.0 / norm
+    for i in range(2):
+        want = eff[i] * (10.0 / (norm + 1e-6))
+        for got, ref in ((opt.exp_avg[i], 0.1 * want), (opt.exp_avg_sq[i], 0.001 * want * want)):
+            off = (got.cpu().double() - ref).abs()
+            assert bool((off <= 2.0 ** -21 * ref.abs() + 2.0 ** -149).all()), (i, float(off.max()))
+        assert bool(torch.isfinite(opt.params[i]).all())
+    assert float(opt.exp_avg[0].view(-1)[7]) > 0.9                          # the outlier is what is left
+
+
+def test_the_factor_enters_a_step_as_a_power_of_two_would(dev):
+    """grad_scale * factor as one product: the same bits as gradients scaled beforehand where both are powers of two, whatever the gradient."""
+    start = [_values((700, 3), 2)]
+    a, b = _adam(start, dev, max_norm=1.0, grad_scales=[64.0]), _adam(start, dev, grad_scales=[64.0])
+    for t in range(3):
+        g = _values((700, 3), 5 + t, 10.0 ** (t - 1))
+        norm = math.sqrt(float(((64.0 * g.double()) ** 2).sum()))
+        a.max_norm = 2.0 ** -6 * (norm + 1e-6)                              # rounded to fp32 the factor is 2^-6
+        a.params[0].grad, b.params[0].grad = g.to(dev), (g * 2.0 ** -6).to(dev)
+        a.step()
+        b.step()
+        assert torch.equal(a.params[0], b.params[0]) and torch.equal(a.exp_avg[0], b.exp_avg[0]) and torch.equal(a.exp_avg_sq[0], b.exp_avg_sq[0]), t

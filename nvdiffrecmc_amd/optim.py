@@ -99,7 +99,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise type(e)('clip_grad_norm_: %s' % e) from None
 
 
-_ADAM_ROW = struct.Struct('=QQQQqfff4xQqQqfiQii').pack          # nvdr_adam_tensor (_lib.NvdrAdamTensor): filling its fields one by one costs 2 us a tensor
+# nvdr_adam_tensor (_lib.NvdrAdamTensor): filling its fields one by one costs 2 us a tensor.  Native mode: a bound or scale beyond fp32 becomes
+# infinite as in the structure (in the standard modes struct raises)
+_ADAM_ROW = struct.Struct('@QQQQqfff4xQqQqfiQii').pack
 _UNBOUNDED = (-math.inf, math.inf, 0, 0, 0, 0)
 
 

@@ -111,3 +111,17 @@ def test_the_factor_enters_a_step_as_a_power_of_two_would(dev):
         a.step()
         b.step()
         assert torch.equal(a.params[0], b.params[0]) and torch.equal(a.exp_avg[0], b.exp_avg[0]) and torch.equal(a.exp_avg_sq[0], b.exp_avg_sq[0]), t
+
+
+# ---- numbers beyond fp32 from the host ---------------------------------------------------------------------------------------------------
+
+def test_bounds_beyond_fp32_do_not_bind(dev):
+    start = [_values((70, 3), 4)]
+    a = _adam(start, dev, clamps=[(-1e39, 1e39)])
+    b = _adam(start, dev)
+    for t in range(2):
+        g = _values((70, 3), t)
+        a.params[0].grad, b.params[0].grad = g.to(dev), g.to(dev)
+        a.step()
+        b.step()
+        assert torch.equal(a.params[0], b.params[0])

@@ -103,6 +103,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 # infinite as in the structure (in the standard modes struct raises)
 _ADAM_ROW = struct.Struct('@QQQQqfff4xQqQqfiQii').pack
 _UNBOUNDED = (-math.inf, math.inf, 0, 0, 0, 0)
+_LEAST_RATE = 2.0 ** -149                                                    # fp32's smallest number
 
 
 class FusedAdam:
@@ -206,8 +207,11 @@ class FusedAdam:
                 bounds = (-math.inf if c[0] is None else c[0], math.inf if c[1] is None else c[1],
                           lo_vec.data_ptr() if lo_vec is not None else 0, lo_vec.numel() if lo_vec is not None else 0,
                           hi_vec.data_ptr() if hi_vec is not None else 0, hi_vec.numel() if hi_vec is not None else 0)
-            # lr_scales[i] == 0 freezes the tensor (the C block's lr_scale 0 means "the plain rate": a zero-initialised block trains)
+            # lr_scales[i] == 0 freezes the tensor (the C block's lr_scale 0 means "the plain rate": a zero-initialised block trains, and a rate
+            # below fp32's range must not become one)
             rate, active = float(self.lr_scales[i]), self.active[i]
+            if 0.0 < rate < _LEAST_RATE:
+                rate = _LEAST_RATE
             rows.append(_ADAM_ROW(p.data_ptr(), g.data_ptr(), self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr(), p.numel(),
                                   self.grad_scales[i] * grad_mult, *bounds, rate or 1.0, bool(self.normalize3[i]),
                                   active.data_ptr() if active is not None else 0, bool(self.zero_grad_after[i]) and active is not None, rate == 0.0))

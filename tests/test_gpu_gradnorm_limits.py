@@ -125,3 +125,14 @@ def test_bounds_beyond_fp32_do_not_bind(dev):
         a.step()
         b.step()
         assert torch.equal(a.params[0], b.params[0])
+
+
+def test_a_rate_below_fp32_is_no_plain_rate(dev):
+    start = [_values((70, 3), 4), _values((9,), 5)]
+    for tiny in (1e-46, 5e-324, 2.0 ** -149):
+        opt = _adam(start, dev, lr_scales=[tiny, 1.0])
+        for q in opt.params:
+            q.grad = torch.ones_like(q)
+        opt.step()
+        assert torch.equal(opt.params[0].cpu(), start[0]) and bool((opt.exp_avg[0] > 0).all())      # (no step that fp32 can hold; the moments go on)
+        assert not torch.equal(opt.params[1].cpu(), start[1])

@@ -26,6 +26,7 @@ struct Lists {
     std::vector<int64_t> n;
     std::vector<uint8_t> type;
     std::vector<Py_ssize_t> irregular;              // tensors whose elements do not fill their memory exactly once
+    std::vector<at::Tensor> held;                   // gradients: the interpreter runs during the call, and another thread may drop a parameter's
     int device = -1;
     int64_t count() const { return (int64_t)n.size(); }
 };
@@ -40,6 +41,7 @@ bool collect(PyObject *seq, bool grads, bool written, Lists &l)
     }
     const size_t most = (size_t)PyList_GET_SIZE(seq);
     l.data.reserve(most); l.n.reserve(most); l.type.reserve(most);
+    if (grads) l.held.reserve(most);
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
         PyObject *item = PyList_GET_ITEM(seq, k);
         if (!THPVariable_Check(item)) {
@@ -75,6 +77,7 @@ bool collect(PyObject *seq, bool grads, bool written, Lists &l)
         l.data.push_back(t.data_ptr());
         l.n.push_back(t.numel());
         l.type.push_back((uint8_t)type);
+        if (grads) l.held.push_back(t);                             // (tensors of a list are held by the list)
         if (written && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     }
     return true;

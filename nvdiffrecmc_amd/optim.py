@@ -199,7 +199,7 @@ class FusedAdam:
                     # a copy would be zeroed instead of the buffer the producer scatter-adds into
                     raise RuntimeError('FusedAdam.step: zero_grad needs a contiguous .grad for parameter %d (the persistent scatter-add buffer itself)' % i)
                 g = g.contiguous()
-                keep.append(g)
+            keep.append(g)                          # (the call runs without the interpreter's lock: another thread may drop p.grad meanwhile)
             bounds, c = _UNBOUNDED, self.clamps[i]
             if c is not None:
                 lo_vec = c[2] if len(c) > 2 else None

@@ -136,3 +136,55 @@ def test_a_rate_below_fp32_is_no_plain_rate(dev):
         opt.step()
         assert torch.equal(opt.params[0].cpu(), start[0]) and bool((opt.exp_avg[0] > 0).all())      # (no step that fp32 can hold; the moments go on)
         assert not torch.equal(opt.params[1].cpu(), start[1])
+
+
+# ---- another thread drops a gradient during the call ---------------------------------------------------------------------------------------
+
+def _entry_that_drops(params, seen):
+    """What another thread may do while a call has released the interpreter's lock; nothing is launched."""
+    def entry(*_):
+        before = torch.cuda.memory_allocated()
+        for p in params:
+            p.grad = None
+        seen.append(before - torch.cuda.memory_allocated())
+        return 0
+    return entry
+
+
+def test_clip_holds_the_gradients_it_scales(dev):
+    import ctypes
+    from nvdiffrecmc_amd import _lib
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    ops, lib = _lib.gradops(), _lib.load()
+    names = ('nvdr_grad_norm', 'nvdr_grad_clip', 'nvdr_grad_norm_workspace', 'nvdr_last_error')
+    own = {n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}
+    params = [torch.nn.Parameter(torch.zeros(1 << 20, device=dev)) for _ in range(3)]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    before, seen = torch.cuda.memory_allocated(), []
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, *([ctypes.c_void_p] * 3), ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p)(
+        _entry_that_drops(params, seen))
+    try:
+        ops.bind(*(ctypes.cast(entry, ctypes.c_void_p).value if n == 'nvdr_grad_clip' else own[n] for n in names), torch._C._cuda_getCurrentRawStream)
+        clip_grad_norm_(params, 1.0)
+    finally:
+        ops.bind(*own.values(), torch._C._cuda_getCurrentRawStream)
+    assert seen == [0]
+    assert torch.cuda.memory_allocated() <= before - (3 << 22) + 512        # ... and no longer (the norm is there)
+
+
+@pytest.mark.parametrize('how', ['plain', 'clipped', 'subset'])
+def test_a_step_holds_the_gradients_it_reads(how, dev, monkeypatch):
+    from types import SimpleNamespace
+    from nvdiffrecmc_amd import _lib
+    opt = _adam([torch.zeros(1 << 20)] * 2, dev, max_norm=None if how == 'plain' else 1.0)
+    for p in opt.params:
+        p.grad = torch.ones_like(p)
+    if how == 'subset':
+        opt.measure_norm()
+    before, seen = torch.cuda.memory_allocated(), []
+    entry = _entry_that_drops(opt.params, seen)
+    monkeypatch.setattr(_lib, 'load', lambda: SimpleNamespace(nvdr_adam_step_clipped=entry, nvdr_adam_step_factor=entry))
+    opt.step(subset=[0, 1] if how == 'subset' else None)
+    assert seen == [0]
+    assert torch.cuda.memory_allocated() <= before - (2 << 22)

@@ -26,14 +26,14 @@ struct Lists {
     std::vector<int64_t> n;
     std::vector<uint8_t> type;
     std::vector<Py_ssize_t> irregular;              // tensors whose elements do not fill their memory exactly once
-    std::vector<at::Tensor> held;                   // gradients: the interpreter runs during the call, and another thread may drop a parameter's
+    std::vector<at::Tensor> held;                   // what a call writes to: another thread may drop a parameter's gradient during the call
     int device = -1;
     int64_t count() const { return (int64_t)n.size(); }
 };
 
-// The gradients in `seq`, a list: tensors, or parameters whose gradients are meant (None is left out).  written: the call is going to write to
-// them: their versions go up, as with any operation in place.  false: an exception is set.
-bool collect(PyObject *seq, bool grads, bool written, Lists &l)
+// The gradients in `seq`, a list: tensors, or parameters whose gradients are meant (None is left out).  hold: with a reference to each.
+// false: an exception is set.
+bool collect(PyObject *seq, bool grads, bool hold, Lists &l)
 {
     if (!PyList_Check(seq)) {
         PyErr_SetString(PyExc_TypeError, "a list is expected");
@@ -41,7 +41,7 @@ bool collect(PyObject *seq, bool grads, bool written, Lists &l)
     }
     const size_t most = (size_t)PyList_GET_SIZE(seq);
     l.data.reserve(most); l.n.reserve(most); l.type.reserve(most);
-    if (grads) l.held.reserve(most);
+    if (hold) l.held.reserve(most);
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
         PyObject *item = PyList_GET_ITEM(seq, k);
         if (!THPVariable_Check(item)) {
@@ -77,8 +77,7 @@ bool collect(PyObject *seq, bool grads, bool written, Lists &l)
         l.data.push_back(t.data_ptr());
         l.n.push_back(t.numel());
         l.type.push_back((uint8_t)type);
-        if (grads) l.held.push_back(t);                             // (tensors of a list are held by the list)
-        if (written && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        if (hold) l.held.push_back(t);
     }
     return true;
 }
@@ -195,6 +194,9 @@ static PyObject *clip(PyObject *, PyObject *args)
         rc = grad_clip_entry(l.data.data(), l.n.data(), l.type.data(), l.count(), code, max_norm, w, size, at, stream);
         Py_END_ALLOW_THREADS
         if (rc) return failed("clip_grad_norm_", rc);
+        // versions go up, as with any operation in place -- not before the call has been accepted
+        for (const at::Tensor &t : l.held)
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
         return THPVariable_Wrap(result);
     });
 }

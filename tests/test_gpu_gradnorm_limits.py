@@ -188,3 +188,52 @@ def test_a_step_holds_the_gradients_it_reads(how, dev, monkeypatch):
     opt.step(subset=[0, 1] if how == 'subset' else None)
     assert seen == [0]
     assert torch.cuda.memory_allocated() <= before - (2 << 22)
+
+
+# ---- versions ------------------------------------------------------------------------------------------------------------------------------
+
+def _with_grads(grads):
+    ps = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+    for p, g in zip(ps, grads):
+        p.grad = g
+    return ps
+
+
+def test_a_refused_clip_leaves_the_versions(dev):
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    a, b, c = torch.ones(5, device=dev), torch.ones(7, device=dev), torch.ones(9, 4, device=dev)
+    cpu, wide, expanded = torch.ones(5), torch.ones(5, device=dev, dtype=torch.float64), torch.ones(1, device=dev).expand(6)
+    lists = {'CPU': [a, b, cpu], 'type': [a, wide], 'twice': [a, b, a], 'overlap': [a, b, b[2:]], 'expanded': [a, expanded, c[:, :2]]}
+    for name, grads in lists.items():
+        versions = [g._version for g in grads]
+        with pytest.raises((RuntimeError, ValueError)):
+            clip_grad_norm_(_with_grads(grads), 0.5)
+        assert [g._version for g in grads] == versions, name
+    bad = torch.tensor([1.0, math.nan], device=dev)
+    versions = a._version, bad._version
+    with pytest.raises(RuntimeError, match='nan'):
+        clip_grad_norm_(_with_grads([a, bad]), 0.5, error_if_nonfinite=True)
+    assert (a._version, bad._version) == versions
+
+
+def test_a_clip_raises_each_version_once(dev):
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    for strided in (False, True):
+        grads = [torch.ones(5, device=dev), torch.ones(9, 4, device=dev)[:, :2] if strided else torch.ones(9, 2, device=dev), torch.ones(300000, device=dev, dtype=torch.bfloat16)]
+        versions = [g._version for g in grads]
+        clip_grad_norm_(_with_grads(grads), 0.5)
+        assert [g._version for g in grads] == [v + 1 for v in versions]
+    # what autograd has saved of a gradient is known to have changed
+    w = torch.ones(4, device=dev, requires_grad=True)
+    g, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    later = (g * g).sum()
+    clip_grad_norm_(_with_grads([g.detach()]), 0.5)
+    with pytest.raises(RuntimeError, match='inplace'):
+        later.backward()
+    with torch.inference_mode():
+        i = torch.ones(5, device=dev)
+    p = torch.nn.Parameter(torch.ones(5, device=dev))
+    with torch.inference_mode():
+        p.grad = i
+        clip_grad_norm_(p, 0.5)
+        assert float(i[0]) < 0.23

@@ -9,6 +9,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <algorithm>
 #include <vector>
 
 #include "nvdr_hip.h"
@@ -80,6 +81,101 @@ bool collect(PyObject *seq, bool grads, bool hold, Lists &l)
         if (hold) l.held.push_back(t);
     }
     return true;
+}
+
+// ---- which tensors share memory ------------------------------------------------------------------------------------------------------------
+// The bytes of a strided tensor: `run` bytes at `at` + sum over the dims of stride * index.  Dims from the longest stride on, none with one index;
+// reach[k]: bytes from the first to behind the last one of the dims from k on.
+struct Bytes {
+    struct Dim { int64_t stride, n; };
+    int64_t at, run;
+    std::vector<Dim> dims;
+    std::vector<int64_t> reach;
+    size_t index;
+};
+
+Bytes bytes_of(const at::Tensor &t, size_t index)              // t has elements
+{
+    Bytes b;
+    const int64_t size = (int64_t)t.element_size();
+    b.at = (int64_t)(uintptr_t)t.data_ptr();
+    b.run = size;
+    b.index = index;
+    for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) != 1) b.dims.push_back({t.stride(d) * size, t.size(d)});
+    std::sort(b.dims.begin(), b.dims.end(), [](const Bytes::Dim &x, const Bytes::Dim &y) { return x.stride < y.stride; });
+    std::vector<Bytes::Dim> kept;
+    for (const Bytes::Dim &d : b.dims) {                           // dims that continue the run or one another are one
+        if (kept.empty() && d.stride == b.run) b.run *= d.n;
+        else if (!kept.empty() && d.stride == kept.back().stride * kept.back().n) kept.back().n *= d.n;
+        else kept.push_back(d);
+    }
+    b.dims.assign(kept.rbegin(), kept.rend());
+    b.reach.assign(b.dims.size() + 1, b.run);
+    for (size_t k = b.dims.size(); k-- > 0;) b.reach[k] = b.reach[k + 1] + (b.dims[k].n - 1) * b.dims[k].stride;
+    return b;
+}
+
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); }       // b > 0
+
+// Have the dims of a from ka on, placed at pa, and those of b from kb on, placed at pb, a byte in common?  Exact: the longer stride is taken apart,
+// index by index where the other reaches, and of two equal strides only the difference of their indices counts, of which one or two are
+// in reach for views that interleave.  Strides that fit one another badly can take many steps: after `steps` of them the answer is yes.
+bool meet(const Bytes &a, size_t ka, int64_t pa, const Bytes &b, size_t kb, int64_t pb, int &steps)
+{
+    if (--steps < 0) return true;
+    if (pa + a.reach[ka] <= pb || pb + b.reach[kb] <= pa) return false;
+    const bool last_a = ka == a.dims.size(), last_b = kb == b.dims.size();
+    if (last_a && last_b) return true;
+    if (!last_a && !last_b && a.dims[ka].stride == b.dims[kb].stride) {
+        const int64_t s = a.dims[ka].stride;
+        const int64_t lo = std::max(1 - a.dims[ka].n, floor_div(pa - pb - b.reach[kb + 1], s) + 1), hi = std::min(b.dims[kb].n - 1, floor_div(pa + a.reach[ka + 1] - pb - 1, s));
+        for (int64_t d = lo; d <= hi; ++d)
+            if (meet(a, ka + 1, pa, b, kb + 1, pb + s * d, steps)) return true;
+        return false;
+    }
+    if (last_a || (!last_b && b.dims[kb].stride > a.dims[ka].stride)) return meet(b, kb, pb, a, ka, pa, steps);
+    const int64_t s = a.dims[ka].stride;
+    const int64_t lo = std::max<int64_t>(0, floor_div(pb - pa - a.reach[ka + 1], s) + 1), hi = std::min(a.dims[ka].n - 1, floor_div(pb + b.reach[kb] - pa - 1, s));
+    for (int64_t i = lo; i <= hi; ++i)
+        if (meet(a, ka + 1, pa + s * i, b, kb, pb, steps)) return true;
+    return false;
+}
+
+bool meets_itself(const Bytes &a, int &steps)
+{
+    for (size_t k = a.dims.size(); k-- > 0;) {
+        const int64_t s = a.dims[k].stride;
+        if (s == 0) return true;
+        for (int64_t d = 1; d < a.dims[k].n && d * s < a.reach[k + 1]; ++d)
+            if (meet(a, k + 1, 0, a, k + 1, d * s, steps)) return true;
+    }
+    return false;
+}
+
+// two tensors that share memory, or one whose own elements do (then *first == *second); false: none
+bool shared(const std::vector<at::Tensor> &tensors, size_t *first, size_t *second)
+{
+    constexpr int STEPS = 1 << 14;
+    std::vector<Bytes> all;
+    all.reserve(tensors.size());
+    for (size_t k = 0; k < tensors.size(); ++k) {
+        if (tensors[k].numel() == 0) continue;
+        all.push_back(bytes_of(tensors[k], k));
+        int steps = STEPS;
+        if (meets_itself(all.back(), steps)) { *first = *second = k; return true; }
+    }
+    std::sort(all.begin(), all.end(), [](const Bytes &x, const Bytes &y) { return x.at < y.at; });
+    for (size_t i = 0; i < all.size(); ++i)
+        for (size_t j = i + 1; j < all.size() && all[j].at < all[i].at + all[i].reach[0]; ++j) {
+            int steps = STEPS;
+            if (meet(all[i], 0, all[i].at, all[j], 0, all[j].at, steps)) {
+                *first = std::min(all[i].index, all[j].index);
+                *second = std::max(all[i].index, all[j].index);
+                return true;
+            }
+        }
+    return false;
 }
 
 PyObject *irregular_list(const Lists &l)
@@ -178,7 +274,12 @@ static PyObject *clip(PyObject *, PyObject *args)
     return guarded([&]() -> PyObject * {
         Lists l;
         if (!collect(seq, grads != 0, true, l)) return nullptr;
-        if (!l.irregular.empty()) return irregular_list(l);
+        if (!l.irregular.empty()) {
+            size_t i, j;
+            if (!shared(l.held, &i, &j)) return irregular_list(l);
+            return i == j ? PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
+                          : PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: two gradients share memory (the same tensor twice, or overlapping views)");
+        }
         if (l.device < 0) Py_RETURN_NONE;
         const c10::DeviceGuard device(at::Device(at::kCUDA, (at::DeviceIndex)l.device));
         void *stream;
@@ -201,6 +302,22 @@ static PyObject *clip(PyObject *, PyObject *args)
     });
 }
 
+// shared(tensors): the positions of two tensors that share memory -- of one whose own elements do: its position twice -- or None (host or GPU: nothing is read)
+static PyObject *shared_pair(PyObject *, PyObject *seq)
+{
+    return guarded([&]() -> PyObject * {
+        std::vector<at::Tensor> tensors;
+        if (!PyList_Check(seq)) return PyErr_Format(PyExc_TypeError, "a list is expected");
+        for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
+            if (!THPVariable_Check(PyList_GET_ITEM(seq, k))) return PyErr_Format(PyExc_TypeError, "tensors are expected");
+            tensors.push_back(THPVariable_Unpack(PyList_GET_ITEM(seq, k)));
+        }
+        size_t i, j;
+        if (!shared(tensors, &i, &j)) Py_RETURN_NONE;
+        return Py_BuildValue("nn", (Py_ssize_t)i, (Py_ssize_t)j);
+    });
+}
+
 // bind(nvdr_grad_norm, nvdr_grad_clip, nvdr_grad_norm_workspace, nvdr_last_error, raw_stream): the library's entries, and where the stream comes from
 static PyObject *bind(PyObject *, PyObject *args)
 {
@@ -219,6 +336,7 @@ static PyObject *bind(PyObject *, PyObject *args)
 
 static PyMethodDef methods[] = {{"norm", norm, METH_VARARGS, "norm(tensors, scales, norm_type, max_norm, out, work)"},
                                 {"clip", clip, METH_VARARGS, "clip(sequence, grads, norm_type, max_norm)"},
+                                {"shared", shared_pair, METH_O, "shared(tensors)"},
                                 {"bind", bind, METH_VARARGS, "bind(nvdr_grad_norm, nvdr_grad_clip, nvdr_grad_norm_workspace, nvdr_last_error, raw_stream)"},
                                 {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_gradops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -65,7 +65,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     the GPU): torch.nn.utils.clip_grad_norm_ with the norm kept in fp64 and two launches for up to 160 tensors (neighbours in memory, like
     the views of a gradient bucket, count as one).  parameters: a tensor or an iterable; those without a gradient are left out.  A norm
     that is infinite or NaN makes the gradients zero or NaN as it does there, unless error_if_nonfinite is set, which waits for the norm
-    and raises before anything is scaled (not inside a graph capture).  max_norm = inf only measures.  Gradients must not share memory."""
+    and raises before anything is scaled (not inside a graph capture).  max_norm = inf only measures.  Gradients that share memory -- the same
+    tensor twice, overlapping views, an expanded tensor -- are refused, and views whose strides take more than
+    2^14 steps to tell apart; views that interleave, like columns of a matrix, are not."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     code, max_norm = _norm_code(norm_type), _max_norm(max_norm)
     if error_if_nonfinite:
@@ -81,12 +83,6 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         # gradients whose elements do not lie side by side: through contiguous copies
         grads = [p.grad for p in parameters if p.grad is not None]
         originals = [grads[i] for i in norm]
-        for g in originals:
-            reach = 0
-            for stride, size in sorted((st, sz) for st, sz in zip(g.stride(), g.shape) if sz != 1):
-                if stride <= reach:
-                    raise RuntimeError('clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place')
-                reach += (size - 1) * stride
         for i in norm:
             grads[i] = grads[i].detach().clone(memory_format=torch.contiguous_format)
         copies = [grads[i] for i in norm]

@@ -237,3 +237,45 @@ def test_a_clip_raises_each_version_once(dev):
         p.grad = i
         clip_grad_norm_(p, 0.5)
         assert float(i[0]) < 0.23
+
+
+# ---- strided gradients that share memory, and that only seem to ----------------------------------------------------------------------------
+
+def test_strided_gradients_that_share_memory_are_refused(dev):
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    h = _values((60, 70), 3)
+    d = h.to(dev)
+    a = d[:, :11]
+    for name, grads in {'the same view twice': [a, a], 'equal views': [d[:, :11], d[:, :11]], 'a buffer and its columns': [d, a], 'columns that overlap': [d[:, :12], d[:, 11:]],
+                        'a row and columns': [d[7], d[:, 69:]]}.items():
+        ps = _with_grads(grads)
+        with pytest.raises(RuntimeError, match='share memory'):
+            clip_grad_norm_(ps, 1e-3)
+        with pytest.raises(RuntimeError, match='share memory'):
+            clip_grad_norm_(ps[::-1], 1e-3)
+        assert torch.equal(d.cpu(), h), name
+    p = torch.nn.Parameter(torch.empty(60, 11, device=dev))
+    p.grad = a
+    with pytest.raises(RuntimeError, match='share memory'):
+        clip_grad_norm_([p, p], 1e-3)
+
+
+def test_strided_gradients_that_interleave_are_scaled(dev):
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    h = _values((6000,), 5)
+    makers = {'rows that pass one another': lambda b: [b.as_strided((2, 3), (3, 2))],                         # offsets 0 2 4 3 5 7
+              'every third': lambda b: [b[0::3], b[1::3], b[2::3]],
+              'a row between columns': lambda b: [b.view(60, 100)[:, :50], b.view(60, 100)[31, 50:], b.view(60, 100)[32:, 50:]]}
+    for name, f in makers.items():
+        d = h.to(dev)
+        grads, want = f(d), f(h.double())
+        norm = math.sqrt(sum(float((x * x).sum()) for x in want))
+        got = clip_grad_norm_(_with_grads(grads), 0.5 * norm)
+        assert abs(got.item() - norm) <= (2.0 ** -24 + 1e-10) * norm
+        factor = 0.5 * norm / (norm + 1e-6)
+        for g, x in zip(grads, want):
+            assert bool(((g.cpu().double() - x * factor).abs() <= 2.0 ** -23 * (x * factor).abs()).all()), name
+        rest = torch.ones(6000, dtype=torch.bool)
+        for x in f(rest):
+            x.fill_(False)
+        assert torch.equal(d.cpu()[rest], h[rest]), name

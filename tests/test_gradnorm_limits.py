@@ -1,6 +1,12 @@
 """The gradient norm, clipping and the clipped Adam step on the host: rows, references, refusals (no GPU needed)."""
+import itertools
 import math
+import random
 import struct
+import time
+
+import pytest
+import torch
 
 from nvdiffrecmc_amd import _lib, optim
 
@@ -20,3 +26,76 @@ def test_a_row_with_numbers_beyond_fp32():
             assert struct.pack('f', got) == struct.pack('f', getattr(plain, name)), (name, value)
     r = _row(hi=1e39)
     assert (r.param, r.grad, r.exp_avg, r.exp_avg_sq, r.n, r.lo, r.hi) == (16, 32, 48, 64, 5, -math.inf, math.inf)
+
+
+# ---- which strided tensors share memory ----------------------------------------------------------------------------------------------------
+
+def _bytes(t, base):
+    """Every byte of every element, one by one."""
+    size, out = t.element_size(), []
+    for idx in itertools.product(*(range(n) for n in t.shape)):
+        at = t.data_ptr() - base + size * sum(i * s for i, s in zip(idx, t.stride()))
+        out += range(at, at + size)
+    return out
+
+
+def _check(tensors, base):
+    got = _lib.gradops().shared(tensors)
+    sets = [_bytes(t, base) for t in tensors]
+    own = [len(set(s)) != len(s) for s in sets]
+    pairs = {(i, j) for i in range(len(sets)) for j in range(i + 1, len(sets)) if set(sets[i]) & set(sets[j])}
+    what = [(t.dtype, t.storage_offset(), t.shape, t.stride()) for t in tensors]
+    if got is None:
+        assert not any(own) and not pairs, what
+    else:
+        assert own[got[0]] if got[0] == got[1] else got in pairs, (what, got)
+    return got
+
+
+def test_shared_memory_of_strided_views_against_every_byte():
+    rng = random.Random(7)
+    buf = torch.zeros(4096, dtype=torch.uint8)
+    base, found = buf.data_ptr(), [0, 0]
+    for _ in range(6000):
+        tensors = []
+        for _ in range(rng.choice([1, 2, 2, 2, 3])):
+            dtype = rng.choice([torch.float32, torch.bfloat16])
+            shape = [rng.choice([1, 2, 3, 4, 5, 0] if rng.random() < 0.1 else [1, 2, 3, 4]) for _ in range(rng.randrange(4))]
+            strides, reach = [], 1
+            for n in shape:                                                 # mostly one inside the other, sometimes anything
+                s = rng.randrange(0, 12) if rng.random() < 0.25 else reach + rng.choice([0, 0, 1, 2, 5])
+                strides.append(s)
+                reach = max(reach, s * n)
+            order = list(range(len(shape)))
+            rng.shuffle(order)
+            tensors.append(buf.view(dtype).as_strided([shape[k] for k in order], [strides[k] for k in order], rng.randrange(24)))
+        found[_check(tensors, base) is None] += 1
+    assert min(found) > 1000, found                                         # both answers were met often
+
+
+def test_shared_memory_of_views_that_a_model_has():
+    w = torch.zeros(60, 70)
+    none = [[w[:, :11], w[:, 11:40], w[:, 40:]], [w[::2], w[1::2]], [w[:30, :35], w[30:, 35:], w[:30, 35:], w[30:, :35]], [w.t()[5:9], w[:, :5], w[3, 9:]],
+            [torch.zeros(8).as_strided((2, 3), (3, 2))], [w[:0], w], [w[:, 3:3], w[:, :]], []]
+    for views in none:
+        assert _check(views, w.data_ptr()) is None
+    a = w[:, :11]
+    assert _check([a, a], w.data_ptr()) == (0, 1)
+    assert _check([w, torch.zeros(3), w[:, :11]], w.data_ptr()) == (0, 2)
+    assert _check([w[:, :12], w[:, 11:]], w.data_ptr()) == (0, 1)
+    assert _check([w[::2], w[1::2], w[7, 3:5]], w.data_ptr()) == (1, 2)
+    assert _check([torch.zeros(1).expand(9)], w.data_ptr()) == (0, 0)
+    assert _check([w, w.view(-1).as_strided((10, 8), (5, 1))], w.data_ptr()) == (1, 1)
+    # large: nothing is enumerated
+    v = torch.empty((1 << 16, 64))
+    views = [v[:, k:k + 2] for k in range(0, 64, 2)]
+    start = time.perf_counter()
+    assert _lib.gradops().shared(views) is None and _lib.gradops().shared(views + [v[5, 63:]]) == (31, 32)
+    assert _lib.gradops().shared([v.t()[k::3] for k in range(3)]) is None and _lib.gradops().shared([v[k::5] for k in range(5)] + [v[4::10]]) == (4, 5)
+    assert time.perf_counter() - start < 2.0
+    c = torch.empty(1 << 24, dtype=torch.bfloat16)
+    assert _lib.gradops().shared([c.as_strided((1 << 20, 2), (3, 1), 0), c.as_strided((1 << 20,), (3,), 2)]) is None
+    with pytest.raises(TypeError, match='list'):
+        _lib.gradops().shared((w,))
+    with pytest.raises(TypeError, match='tensors'):
+        _lib.gradops().shared([1])

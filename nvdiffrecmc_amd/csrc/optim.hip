@@ -250,6 +250,8 @@ __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, do
 // tensors needs no launch for it: the kernel that finishes the norm prepares the step and moves the counter.)
 __global__ void adam_advance_kernel(int *state, double beta1d, double beta2d) { adam_advance(state, beta1d, beta2d); }
 
+static bool adam_overlap(const float *a, int64_t na, const float *b, int64_t nb) { return na > 0 && nb > 0 && a < b + nb && b < a + na; }
+
 // checks the tensors of a step and deals the workgroups; *blocks_out = how many, *stream_out = whether the moments go past the caches (a sparse
 // texture does not count: what a step touches of it is few tiles, and known to the device alone)
 static int adam_table(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps, const int *state, AdamTable &tab, unsigned *blocks_out,
@@ -264,8 +266,13 @@ static int adam_table(const nvdr_adam_tensor *tensors, int n_tensors, double lr,
     for (int k = 0; k < n_tensors; ++k) {
         const nvdr_adam_tensor &t = tensors[k];
         NVDR_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq && t.n >= 0, "adam_step: tensor %d has a NULL buffer", k);
-        for (int j = 0; j < k; ++j)
-            NVDR_REQUIRE(tensors[j].param != t.param || !t.n || !tensors[j].n, "adam_step: tensors %d and %d are the same (two workgroups would update it)", j, k);
+        for (int j = 0; j < k; ++j) {
+            const nvdr_adam_tensor &o = tensors[j];
+            const float *const mine[3] = {t.param, t.exp_avg, t.exp_avg_sq}, *const others[3] = {o.param, o.exp_avg, o.exp_avg_sq};
+            for (int a = 0; a < 9; ++a)
+                NVDR_REQUIRE(!adam_overlap(mine[a / 3], t.n, others[a % 3], o.n), "adam_step: tensors %d and %d are the same or overlap (two workgroups would update them)", j, k);
+            NVDR_REQUIRE(!(o.zero_grad || t.zero_grad) || !adam_overlap(o.grad, o.n, t.grad, t.n), "adam_step: tensors %d and %d share a gradient that zero_grad clears", j, k);
+        }
         NVDR_REQUIRE(!t.lo_vec || t.lo_vec_n > 0, "adam_step: tensor %d: lo_vec without length", k);
         NVDR_REQUIRE(!t.hi_vec || t.hi_vec_n > 0, "adam_step: tensor %d: hi_vec without length", k);
         NVDR_REQUIRE(!t.normalize3 || t.n % 3 == 0, "adam_step: tensor %d: normalize3 needs a multiple of three elements", k);

@@ -99,3 +99,39 @@ def test_shared_memory_of_views_that_a_model_has():
         _lib.gradops().shared((w,))
     with pytest.raises(TypeError, match='tensors'):
         _lib.gradops().shared([1])
+
+
+# ---- tensors of a step that share memory -----------------------------------------------------------------------------------------------------
+
+def _step(*rows, m=(1, 1), v=(2, 2)):
+    """nvdr_adam_step_factor on rows of (parameter, gradient, elements, zero_grad): addresses that nobody reads, since the last row is refused for its
+    rate if for nothing else."""
+    A, lib = 1 << 30, _lib.load()
+    tab = b''.join(optim._ADAM_ROW(p, g, m[k] * A + k * 4096, v[k] * A + k * 4096, n, 1.0, -math.inf, math.inf, 0, 0, 0, 0, -1.0 if k == len(rows) - 1 else 1.0, 0, 3 * A if z else 0, z, 0)
+                   for k, (p, g, n, z) in enumerate(rows))
+    assert lib.nvdr_adam_step_factor(tab, len(rows), 1e-3, 0.9, 0.999, 1e-8, A, 1, None, None) == -1
+    return lib.nvdr_last_error().decode()
+
+
+def test_a_step_refuses_tensors_that_overlap():
+    B, G = 1 << 20, 1 << 22
+    apart = [(B, G, 12, 0), (B + 48, G + 48, 12, 0)]
+    assert 'lr_scale' in _step(*apart) and 'lr_scale' in _step(*apart[::-1])
+    assert 'lr_scale' in _step((B, G, 12, 0), (B, G, 0, 0))                 # nothing of nothing
+    for other in (B, B + 44, B + 16, B - 44):
+        for n in (12, 15):
+            assert 'tensors 0 and 1 are the same or overlap' in _step((B, G, 12, 0), (other, G + 4096, n, 0))
+    assert 'tensors 0 and 2 are the same' in _step((B, G, 12, 0), (B + 4096, G + 4096, 12, 0), (B + 8, G + 8192, 12, 0), m=(1, 1, 1), v=(2, 2, 2))
+    A = 1 << 30
+    assert 'are the same or overlap' in _step((B, G, 3000, 0), (B + (1 << 19), G + (1 << 19), 3000, 0))          # (the moments, 4096 bytes apart)
+    assert 'are the same or overlap' in _step((B, G, 12, 0), (A, G + 4096, 12, 0))                               # a parameter in another one's moments
+
+
+def test_a_step_refuses_a_shared_gradient_that_it_would_clear():
+    B, G = 1 << 20, 1 << 22
+    far = B + 4096
+    assert 'lr_scale' in _step((B, G, 12, 0), (far, G, 12, 0))              # only read
+    assert 'lr_scale' in _step((B, G, 12, 1), (far, G + 48, 12, 1))
+    for z in ((1, 0), (0, 1), (1, 1)):
+        for at in (G, G + 44, G - 44):
+            assert 'share a gradient that zero_grad clears' in _step((B, G, 12, z[0]), (far, at, 12, z[1]))

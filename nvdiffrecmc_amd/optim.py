@@ -102,10 +102,18 @@ _UNBOUNDED = (-math.inf, math.inf, 0, 0, 0, 0)
 _LEAST_RATE = 2.0 ** -149                                                    # fp32's smallest number
 
 
+def _check_bounds(clamps, device):
+    """Per-channel bounds are read by the kernel where they lie."""
+    for i, c in enumerate(clamps):
+        for v in (c[2:4] if c is not None else ()):
+            if v is not None and (v.dtype != torch.float32 or v.device != device or not v.is_contiguous() or v.numel() == 0):
+                raise ValueError('FusedAdam: the per-channel bounds of parameter %d must be contiguous fp32 tensors on its GPU' % i)
+
+
 class FusedAdam:
     """params: list of tensors (requires_grad, contiguous fp32, on one GPU).
     clamps[i]: None or (lo, hi[, lo_vec[, hi_vec]]) with lo / hi floats or None and lo_vec / hi_vec optional per-channel bounds
-    (device tensors: element e is bounded by lo_vec[e % len(lo_vec)] / hi_vec[e % len(hi_vec)]; Texture2D.clamp_).
+    (fp32 tensors on the same GPU: element e is bounded by lo_vec[e % len(lo_vec)] / hi_vec[e % len(hi_vec)]; Texture2D.clamp_).
     grad_scales[i]: factor applied to the gradient of parameter i inside the update (p.grad itself is left alone).
     lr_scales[i]: learning rate of parameter i relative to lr (the reference runs three Adams with position / material / light
     rates, train.py:336-356).  normalize3[i]: renormalise every texel of three channels after the clamps (the normal map).
@@ -126,6 +134,7 @@ class FusedAdam:
                 raise ValueError('FusedAdam: parameters must be contiguous fp32 tensors on the GPU')
         self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
         self.clamps = list(clamps) if clamps is not None else [None] * len(self.params)
+        _check_bounds(self.clamps, self.params[0].device)
         self.grad_scales = list(grad_scales) if grad_scales is not None else [1.0] * len(self.params)
         self.lr_scales = list(lr_scales) if lr_scales is not None else [1.0] * len(self.params)
         self.normalize3 = list(normalize3) if normalize3 is not None else [False] * len(self.params)

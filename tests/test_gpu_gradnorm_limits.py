@@ -279,3 +279,11 @@ def test_strided_gradients_that_interleave_are_scaled(dev):
         for x in f(rest):
             x.fill_(False)
         assert torch.equal(d.cpu()[rest], h[rest]), name
+
+
+def test_bounds_on_the_host_are_refused(dev):
+    bound = torch.tensor([0.0, 0.1, 0.2])
+    for c in ((None, None, bound), (None, None, None, bound.double().to(dev))):
+        with pytest.raises(ValueError, match='bounds of parameter 0'):
+            _adam([torch.zeros(5, 3)], dev, clamps=[c])
+    _adam([torch.zeros(5, 3)], dev, clamps=[(None, None, bound.to(dev))])

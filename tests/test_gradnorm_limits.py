@@ -135,3 +135,13 @@ def test_a_step_refuses_a_shared_gradient_that_it_would_clear():
     for z in ((1, 0), (0, 1), (1, 1)):
         for at in (G, G + 44, G - 44):
             assert 'share a gradient that zero_grad clears' in _step((B, G, 12, z[0]), (far, at, 12, z[1]))
+
+
+def test_per_channel_bounds_are_checked():
+    dev = torch.device('cpu')
+    good = torch.tensor([0.0, 0.1, 0.2])
+    optim._check_bounds([None, (0.0, 1.0), (None, None, good), [None, 1.0, None, good], (0.0, 1.0, None, None), (0.0, 1.0, good, good[1:])], dev)
+    for bad in (good.double(), good.half(), good.long(), torch.zeros(6)[::2], torch.zeros(1).expand(3), good[:0], torch.empty(3, device='meta')):
+        for c in ((0.0, 1.0, bad), (0.0, 1.0, None, bad), [0.0, 1.0, good, bad]):
+            with pytest.raises(ValueError, match='bounds of parameter 1'):
+                optim._check_bounds([None, c], dev)

@@ -130,8 +130,8 @@ class FusedAdam:
         if not 1 <= len(self.params) <= 8:
             raise ValueError('FusedAdam: 1..8 parameter tensors')
         for p in self.params:
-            if p.dtype != torch.float32 or not p.is_contiguous() or not p.is_cuda:
-                raise ValueError('FusedAdam: parameters must be contiguous fp32 tensors on the GPU')
+            if p.dtype != torch.float32 or not p.is_contiguous() or not p.is_cuda or p.device != self.params[0].device:
+                raise ValueError('FusedAdam: parameters must be contiguous fp32 tensors on the GPU, all on the same one')
         self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
         self.clamps = list(clamps) if clamps is not None else [None] * len(self.params)
         _check_bounds(self.clamps, self.params[0].device)

@@ -4,6 +4,7 @@ import math
 import random
 import struct
 import time
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -145,3 +146,12 @@ def test_per_channel_bounds_are_checked():
         for c in ((0.0, 1.0, bad), (0.0, 1.0, None, bad), [0.0, 1.0, good, bad]):
             with pytest.raises(ValueError, match='bounds of parameter 1'):
                 optim._check_bounds([None, c], dev)
+
+
+def test_parameters_lie_on_one_gpu():
+    def fake(index, **kw):
+        return SimpleNamespace(**dict(dict(dtype=torch.float32, is_contiguous=lambda: True, is_cuda=True, device=torch.device('cuda', index)), **kw))
+    for params in ([fake(0), fake(1)], [fake(1), fake(0)], [fake(0), fake(0, is_cuda=False, device=torch.device('cpu'))], [fake(0, dtype=torch.float16)],
+                   [fake(0, is_contiguous=lambda: False)]):
+        with pytest.raises(ValueError, match='on the GPU'):
+            optim.FusedAdam(params)

@@ -31,12 +31,12 @@ SOURCES = [
     'exchange.hip',
 ]
 
-# -ffp-contract=off: the sampling math must round exactly like the CPU oracle
-# (see include/nvdr_detmath.h); fused operations are written as explicit fmaf.
 # nvdr_grad_norm / nvdr_grad_clip for lists of Python tensors: a CPython extension against the installed torch (host code only)
 GRADOPS_SOURCE = os.path.join(CSRC, 'gradops.cpp')
 GRADOPS = os.path.join(BUILD, '_gradops.so')
 
+# -ffp-contract=off: the sampling math must round exactly like the CPU oracle
+# (see include/nvdr_detmath.h); fused operations are written as explicit fmaf.
 # -packed-fp32-ops: the compiler makes v_pk_add / mul / fma_f32 from ordinary float code at -O3, and some of their forms have given wrong
 # results now and then on MI355X; the target feature is taken away for every source (the host pass warns that it does not know it).
 FLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
@@ -59,58 +59,76 @@ def _deps_mtime():
     return m
 
 
-def _compile(src, force, hdr_mtime, verbose):
-    obj = os.path.join(BUILD, os.path.splitext(src)[0] + '.o')
-    sp = os.path.join(CSRC, src)
-    if (not force and os.path.exists(obj) and os.path.getmtime(obj) > os.path.getmtime(sp)
-            and os.path.getmtime(obj) > hdr_mtime):
-        return obj, False
-    cmd = [_hipcc()] + FLAGS + ['-c', sp, '-o', obj]
+def _current(out, recipe, newest):
+    """Is `out` younger than what it is made from, and was it made by this recipe (the command line and the versions behind it)?"""
+    try:
+        with open(out + '.recipe') as f:
+            return os.path.getmtime(out) > newest and f.read() == recipe
+    except OSError:
+        return False
+
+
+def _make(what, cmd, out, recipe, verbose):
     if verbose:
         print(' '.join(cmd), flush=True)
+    if os.path.exists(out + '.recipe'):
+        os.remove(out + '.recipe')              # (what a failed command leaves is not current)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError('hipcc failed for %s:\n%s\n%s' % (src, r.stdout, r.stderr))
+        raise RuntimeError('%s failed:\n%s\n%s' % (what, r.stdout, r.stderr))
     if verbose and r.stderr.strip():
         print(r.stderr, file=sys.stderr)
+    with open(out + '.recipe', 'w') as f:
+        f.write(recipe)
+
+
+def _version(exe):
+    return subprocess.run([exe, '--version'], capture_output=True, text=True).stdout
+
+
+def _compile(src, force, hdr_mtime, version, verbose):
+    obj = os.path.join(BUILD, os.path.splitext(src)[0] + '.o')
+    sp = os.path.join(CSRC, src)
+    cmd = [_hipcc()] + FLAGS + ['-c', sp, '-o', obj]
+    recipe = '\n'.join(cmd + [version])
+    if not force and _current(obj, recipe, max(os.path.getmtime(sp), hdr_mtime)):
+        return obj, False
+    _make('hipcc for ' + src, cmd, obj, recipe, verbose)
     return obj, True
 
 
 def build(force=False, verbose=False):
-    """Compile every HIP translation unit for gfx950 and link libnvdr_hip.so.  Returns its path."""
+    """Compile every HIP translation unit for gfx950 and link libnvdr_hip.so.  Returns its path.  What is there already stays when it was made from
+    these sources by these commands, flags and versions."""
     os.makedirs(BUILD, exist_ok=True)
     hdr_mtime = _deps_mtime()
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     missing = [s for s in SOURCES if s not in srcs]
     if missing:
         raise RuntimeError('missing HIP sources: %s' % missing)
+    version = _version(_hipcc())
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        res = list(ex.map(lambda s: _compile(s, force, hdr_mtime, verbose), srcs))
+        res = list(ex.map(lambda s: _compile(s, force, hdr_mtime, version, verbose), srcs))
     objs = [o for o, _ in res]
-    if force or any(c for _, c in res) or not os.path.exists(LIB):
-        cmd = [_hipcc(), '--offload-arch=' + ARCH, '-shared', '-fPIC'] + objs + ['-ldl', '-o', LIB]
-        if verbose:
-            print(' '.join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError('link failed:\n%s\n%s' % (r.stdout, r.stderr))
-    if force or not os.path.exists(GRADOPS) or os.path.getmtime(GRADOPS) < max(os.path.getmtime(GRADOPS_SOURCE), hdr_mtime):
-        _build_gradops(verbose)
+    cmd = [_hipcc(), '--offload-arch=' + ARCH, '-shared', '-fPIC'] + objs + ['-ldl', '-o', LIB]
+    recipe = '\n'.join(cmd + [version])
+    if force or any(c for _, c in res) or not _current(LIB, recipe, max(os.path.getmtime(o) for o in objs)):
+        _make('link', cmd, LIB, recipe, verbose)
+    _build_gradops(force, hdr_mtime, verbose)
     return LIB
 
 
-def _build_gradops(verbose):
+def _build_gradops(force, hdr_mtime, verbose):
     import sysconfig
     import torch
     from torch.utils import cpp_extension
-    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI,
+    cxx = os.environ.get('CXX', 'g++')
+    cmd = [cxx, '-O2', '-std=c++17', '-fPIC', '-shared', '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI,
            '-I' + os.path.join(ROOT, 'include'), '-I' + sysconfig.get_paths()['include']] + ['-I' + d for d in cpp_extension.include_paths()]
     cmd += [GRADOPS_SOURCE, '-o', GRADOPS] + ['-L' + d for d in cpp_extension.library_paths()] + ['-ltorch_python', '-ltorch_cpu', '-lc10']
-    if verbose:
-        print(' '.join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError('g++ failed for gradops.cpp:\n%s\n%s' % (r.stdout, r.stderr))
+    recipe = '\n'.join(cmd + [torch.__version__, sys.version, _version(cxx)])
+    if force or not _current(GRADOPS, recipe, max(os.path.getmtime(GRADOPS_SOURCE), hdr_mtime)):
+        _make('g++ for gradops.cpp', cmd, GRADOPS, recipe, verbose)
 
 
 if __name__ == '__main__':

@@ -49,12 +49,8 @@
 #ifndef NVDR_BWD_ROLL
 #define NVDR_BWD_ROLL 1
 #endif
-// measurements only (variants): 1 = no light-gradient records at all, 2 = none + round-robin groups, 3 = unsorted in-place records + round-robin
 #ifndef NVDR_CDF_GUIDE
 #define NVDR_CDF_GUIDE 1          // CDF inversion through guide tables (0: the reference's bisection; A/B)
-#endif
-#ifndef NVDR_LG_EXPERIMENT
-#define NVDR_LG_EXPERIMENT 0
 #endif
 #ifndef NVDR_GEN_OCC
 #define NVDR_GEN_OCC 4   // 128 VGPRs (14 dwords spilled) instead of 150: 4 waves per SIMD, -3 % time
@@ -1118,7 +1114,7 @@ __global__ void __launch_bounds__(256, BACKWARD ? NVDR_SHADE_OCC : 1) env_shade_
     // that the stream slots it has consumed form one growing range -- the space its light-gradient records go to (below).
     const unsigned wave_id = (unsigned)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (blockDim.x >> 6) + wave));
     unsigned grp_first = wave_id, grp_last = n_groups, grp_step = waves_total;
-    if (BACKWARD && NVDR_LG_EXPERIMENT != 2 && NVDR_LG_EXPERIMENT != 3) {
+    if (BACKWARD) {
         const unsigned per_wave = (n_groups + waves_total - 1) / waves_total;
         grp_first = min(wave_id * per_wave, n_groups);
         grp_last = min(grp_first + per_wave, n_groups);
@@ -1230,14 +1226,7 @@ __global__ void __launch_bounds__(256, BACKWARD ? NVDR_SHADE_OCC : 1) env_shade_
             }
             // No atomic leaves the workgroup in records mode (21 M addends per 8-view launch were 63 M memory-side fp32 atomics):
             // the addends of this round go to the band blocks, light-sampled ones first, in lane order
-#if NVDR_LG_EXPERIMENT == 0
             if (BACKWARD && p.lg_records) rb.emit(p, lane, lg_hasA, lg_recA, lg_hasB, lg_recB, lg_cnt);
-#elif NVDR_LG_EXPERIMENT == 3           // records written in place, unsorted (what the shading kernel cost before the band blocks)
-            if (BACKWARD && p.lg_records) {
-                if (lg_hasA) p.rays[rA] = lg_recA;
-                if (lg_hasB) p.rays[rB] = lg_recB;
-            }
-#endif
         }
         if (BACKWARD) rb.free_end = (grp + 1u) * gs;    // the rays of this group have all been read: its slots may hold records now
 
@@ -1753,9 +1742,6 @@ __global__ void __launch_bounds__(256, BACKWARD ? NVDR_SHADE_OCC : 1) env_shade_
 
 #define NVDR_LG_THREADS 1024
 #define NVDR_LG_PER_BAND_MAX_SLOTS (320ll << 20)    // launches of up to this many stream slots (ten views of 512^2 x 64 spp) deal the CUs to the bands.  Round 4, fp32 accumulators: -13 % / -6 % / -2 % / +-0 of the backward shading + gather time at 1 / 2 / 4 / 8 views of 512^2 (then: 192 Mi slots).  Round 6, with the fp64 build these launches get: -2.3 % at eight views of 512^2 (256 Mi slots), +1.3 % at eight of 800^2 (625 Mi) -- session 27
-#ifndef NVDR_LG_SKIP
-#define NVDR_LG_SKIP 0                   // timing-only A/B (wrong results): bit 0 no LDS adds, bit 1 no record loads, bit 2 no partial row written, bit 3 no zeroing of the accumulators
-#endif
 // (Round 6, measured and dropped, profiles/r06_ab_gather_batched_adds.md: all compare-and-swaps of a step issued as one batch, verdicts afterwards -- the
 // gather 72 -> 119 us at one view, 275 -> 466 at eight: a swap whose word was read a batch earlier fails far more often on the sampler's hot texels.)
 #ifndef NVDR_LG_NB
@@ -1806,7 +1792,7 @@ __global__ void __launch_bounds__(NVDR_LG_THREADS) light_grad_block_kernel(uint1
     for (int band = band_first; band < band_last; ++band) {
         const int t_lo = band * band_texels, t_hi = min(t_lo + band_texels, n_texels);
         const int n_acc = (t_hi - t_lo) * 3;
-        if (!(NVDR_LG_SKIP & 8)) for (int i = threadIdx.x; i < n_acc; i += NVDR_LG_THREADS) { if (F64) lg_acc64[i] = 0.0; else lg_acc[i] = 0.0f; }
+        for (int i = threadIdx.x; i < n_acc; i += NVDR_LG_THREADS) { if (F64) lg_acc64[i] = 0.0; else lg_acc[i] = 0.0f; }
         __syncthreads();
         // fp32 add to LDS.  NOT ds_add_f32: gfx950 executes that at 0.8 lane-operations per CU and nanosecond, twenty times slower
         // than its integer LDS atomics (tools/ubench/lds_atomic.hip, profiles/r03_lds_atomic_ubench.txt) -- it was 0.55 ms of the
@@ -1870,21 +1856,16 @@ __global__ void __launch_bounds__(NVDR_LG_THREADS) light_grad_block_kernel(uint1
 #pragma unroll
                 for (int q = 0; q < NVDR_LG_NB; ++q) {
                     cc[2 * q] = none; cc[2 * q + 1] = none;
-                    if (!(NVDR_LG_SKIP & 2)) {
-                        if (lane < ff[q]) cc[2 * q] = recs[(bb[q] << 7) + lane];
-                        if (lane + 64u < ff[q]) cc[2 * q + 1] = recs[(bb[q] << 7) + 64u + lane];
-                    } else if (lane < ff[q]) cc[2 * q] = make_float4(1.0f, 1.0f, 1.0f, __int_as_float(t_lo + (int)((bb[q] * 64u + lane) % (unsigned)(t_hi - t_lo))));
+                    if (lane < ff[q]) cc[2 * q] = recs[(bb[q] << 7) + lane];
+                    if (lane + 64u < ff[q]) cc[2 * q + 1] = recs[(bb[q] << 7) + 64u + lane];
                 }
 #pragma unroll
-                for (int q = 0; q < 2 * NVDR_LG_NB; ++q) {
-                    if (!(NVDR_LG_SKIP & 1)) add(cc[q]);
-                    else asm volatile("" :: "v"(cc[q].x), "v"(cc[q].w));
-                }
+                for (int q = 0; q < 2 * NVDR_LG_NB; ++q) add(cc[q]);
             }
         }
         __syncthreads();
         float *out = partials + (int64_t)g * n_texels * 3 + (int64_t)t_lo * 3;
-        if (!(NVDR_LG_SKIP & 4)) for (int i = threadIdx.x; i < n_acc; i += NVDR_LG_THREADS) out[i] = F64 ? (float)lg_acc64[i] : lg_acc[i];
+        for (int i = threadIdx.x; i < n_acc; i += NVDR_LG_THREADS) out[i] = F64 ? (float)lg_acc64[i] : lg_acc[i];
         __syncthreads();
     }
 }

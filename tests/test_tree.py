@@ -32,3 +32,8 @@ def test_tools_that_are_named_exist():
     named = {(os.path.relpath(f, ROOT), m) for f in files for m in re.findall(r'\btools/[\w/]+\.(?:py|sh|hip|c|txt)\b', open(f).read())}
     assert len(named) > 20
     assert not sorted((f, m) for f, m in named if not os.path.exists(os.path.join(ROOT, m)))
+
+
+def test_no_build_switch_leaves_work_out():
+    """A build that skips work to time the rest has no place in the sources."""
+    assert not [f for f in _files('.hip', '.h', '.cpp') if re.search(r'#define \w*(SKIP|EXPERIMENT)\w*', open(f).read())]

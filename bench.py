@@ -68,7 +68,7 @@ import time
 ROOT = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, ROOT)
 
-from tools.bench_parts import (PRESETS, DOMINANT, GEOMETRY_NOTE, TEXTURE_NOTE, BENCH_LR_POS, HBM_PEAK_GBS, VALU_PEAK_TLANEOPS, make_step, algorithmic_bytes,
+from tools.bench_parts import (brief_line, PRESETS, DOMINANT, GEOMETRY_NOTE, TEXTURE_NOTE, BENCH_LR_POS, HBM_PEAK_GBS, VALU_PEAK_TLANEOPS, make_step, algorithmic_bytes,
                                cpu_baseline, cpu_baseline_torch, collect_pmc, find_kernel, valu_figures, mem_figures, other_config_object, adam_object,
                                init_world1, exchange_object, flat_scaling_keys, bvh_policy_note, collect_extras, extras_child, _stdout_to_stderr, _free_port)
 
@@ -109,6 +109,7 @@ def parse_args():
     ap.add_argument('--extras-timeout', type=int, default=420, help='seconds the extra objects of the default N = 1 line may take together (they run in a child process)')
     ap.add_argument('--extras-child', default=None, help=argparse.SUPPRESS)
     ap.add_argument('--no-validation', action='store_true', help='skip the `validation_n32` object (n_samples_x = 32, one view) of the default N = 1 line')
+    ap.add_argument('--full-line', action='store_true', help='print every detail on the line; without it a long line is shortened and the whole object goes to stderr')
     ap.add_argument('--graph', choices=('auto', 'on', 'off'), default='auto',
                     help='capture the iteration in HIP graphs (auto: when a rank renders <= 2 views -- the launch-bound regime -- or there are several ranks)')
     return ap.parse_args()
@@ -482,7 +483,11 @@ def run(args):
             with _stdout_to_stderr():
                 if _d.is_initialized():
                     _d.destroy_process_group()
-        print(json.dumps(out), flush=True)
+        # the line itself stays short enough to be read whole by whoever keeps the end of the output; everything goes to stderr
+        line = json.dumps(out) if args.full_line else brief_line(out)
+        if line != json.dumps(out):
+            print(json.dumps(out), file=sys.stderr, flush=True)
+        print(line, flush=True)
     if dist is not None:
         dist.barrier()
         with _stdout_to_stderr():

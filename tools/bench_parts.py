@@ -28,6 +28,45 @@ VALU_PEAK_TLANEOPS = N_CUS * SIMDS_PER_CU * LANES_PER_SIMD * CLOCK_GHZ * 1e9 / 1
 # 1e-5 keeps the mesh a mesh over the few hundred iterations of a bench run (< 0.003 units of drift); the work per iteration does not depend on it.
 BENCH_LR_POS = 1e-5
 
+LINE_LIMIT = 7000          # bytes of the JSON line: whoever keeps the end of a program's output keeps some 8 KB of it
+
+
+def brief_line(out, limit=LINE_LIMIT):
+    """`out` as one JSON line of at most `limit` bytes.  A shorter object is written as it is.  Of a longer one the numbers of the objects inside are
+    rounded to six digits and their long texts left out, then the most detailed parts go, one by one; the keys and numbers of the object itself and the
+    plain entries of `config` and `roofline` always stay."""
+    line = json.dumps(out)
+    if len(line) <= limit:
+        return line
+
+    def thin(v, text):
+        if isinstance(v, dict):
+            return {k: thin(x, text) for k, x in v.items() if not (isinstance(x, str) and len(x) > text)}
+        if isinstance(v, list):
+            return [thin(x, text) for x in v]
+        return float('%.6g' % v) if isinstance(v, float) and math.isfinite(v) else v
+
+    out = {k: thin(v, 250 if k == 'config' else 60) if isinstance(v, dict) else v for k, v in out.items()}
+    out['left_out'] = ['long texts']
+
+    def drop(holder, k, name):
+        del holder[k]
+        out['left_out'].append(name)
+
+    detail = [(h, k, '%s.%s' % (n, k)) for n, h in out.items() if isinstance(h, dict) for k, x in h.items() if isinstance(x, (dict, list))]
+    detail.sort(key=lambda d: -len(json.dumps(d[0][d[1]])))
+    for d in detail:
+        if len(json.dumps(out)) <= limit:
+            break
+        drop(*d)
+    whole = sorted((k for k, v in out.items() if isinstance(v, dict) and k not in ('config', 'roofline')), key=lambda k: -len(json.dumps(out[k])))
+    for k in whole:
+        if len(json.dumps(out)) <= limit:
+            break
+        drop(out, k, k)
+    return json.dumps(out)
+
+
 PRESETS = {
     # lock_pos / tex_res: the config's own keys (configs/bob.json:6,14; spot_metal.json; nerf_lego / nerfactor_hotdog train the geometry:
     # their second pass runs DLMesh with v_pos as a parameter, geometry/dlmesh.py:28-38)

@@ -9,7 +9,7 @@ if [ -z "$SKIP_TESTS" ]; then
 echo "== gpu tests"; timeout 1800 python -m pytest tests -q -m gpu 2>&1 | tail -3
 echo "== smoke"; timeout 300 python -c "import __graft_entry__ as g; g.smoke()" 2>&1 | tail -1
 fi
-echo "== bench (driver's command)"; SECONDS=0; timeout 1200 python bench.py --gpus 1 --pmc-keep $O 2> $O/bench_err.log | tail -1 > $O/bench_bob512_n1.json; echo "wall $SECONDS s"
+echo "== bench (driver's command)"; SECONDS=0; timeout 1200 python bench.py --gpus 1 --full-line --pmc-keep $O 2> $O/bench_err.log | tail -1 > $O/bench_bob512_n1.json; echo "wall $SECONDS s"
 python - <<PY
 import json; d=json.load(open('$O/bench_bob512_n1.json'))
 print(d['value'], d['ms_per_step'], d['median_ms_per_step'], d['iters_per_sec'], d['config'].get('ms_per_step_cached_visibility'))
@@ -48,7 +48,7 @@ one oneview_dmtet64_800_unlocked_graph_on --config dmtet64_800 --batch 1 --graph
 one eightviews_dmtet800_unlocked --config dmtet800 --steps 30 --warmup 6
 one eightviews_dmtet800_locked --config dmtet800 --lock-pos on --steps 30 --warmup 6
 one eightviews_bob512_graph_on --graph on
-full() { name=$1; shift; timeout 600 python bench.py "$@" --no-cpu-baseline --no-one-view --pmc-keep $O 2>/dev/null | tail -1 > $O/bench_$name.json
+full() { name=$1; shift; timeout 600 python bench.py "$@" --full-line --no-cpu-baseline --no-one-view --pmc-keep $O 2>/dev/null | tail -1 > $O/bench_$name.json
   python -c "import json; d=json.load(open('$O/bench_$name.json')); r=d['roofline']; print('$name', d['ms_per_step'], d['median_ms_per_step'], r['kernel_ms_hip_events'], r['frac'], r.get('hbm', {}).get('hbm_frac'), r.get('l2', {}).get('l2_hit'))"; }
 full dmtet64_800_n1 --config dmtet64_800 --steps 8 --warmup 3
 full dmtet800_n1 --config dmtet800 --steps 10 --warmup 3

@@ -438,7 +438,11 @@ static bool gn_one(const GradList &l, int64_t bytes) { return l.count <= NVDR_GN
 // in doubles: the parts, the words of the last launch, the factor of nvdr_grad_clip.  (A launch ends with the list or with a full table; the split by
 // the number of chunks needs more than 2^31 of them, 8 TB.)
 static int64_t gn_part_room(int64_t count) { return ((count + NVDR_GN_TENSORS - 1) / NVDR_GN_TENSORS + 1) * NVDR_GN_GRID; }
-static int64_t gn_workspace(const GradList &l, bool clip) { return clip && gn_one(l, gn_bytes(l)) ? 0 : gn_part_room(l.count) + 2 * NVDR_GN_GRID + 1; }
+static int64_t gn_workspace(const GradList &l, bool clip)
+{
+    // (a long list is not walked for its bytes)
+    return clip && l.count <= NVDR_GN_ONE_TENSORS && gn_one(l, gn_bytes(l)) ? 0 : gn_part_room(l.count) + 2 * NVDR_GN_GRID + 1;
+}
 
 static int gn_check(const GradList &l, int norm_type, double max_norm, bool clip, const double *workspace, int64_t workspace_len, const float *norm, const char *who)
 {
@@ -556,12 +560,11 @@ static GradKeys gn_keys()
     return {mix(at), mix(at + 1)};          // (of two different counts: never equal, so that erased words do not open)
 }
 
-// the launches of the norm; finish: the last one writes it
+// the launches of the norm; finish: the last one writes it.  tab: as the last one had it
 template <int P>
-static int gn_parts(const GradList &l, int64_t bytes, double *part, bool finish, const GradOut &out, GradLaunches &g, hipStream_t st)
+static int gn_parts(const GradList &l, int64_t bytes, double *part, bool finish, const GradOut &out, GradLaunches &g, GradTable &tab, hipStream_t st)
 {
     unsigned long long *words = (unsigned long long *)(part + gn_part_room(l.count));
-    GradTable tab;
     int64_t at = 0, left = bytes;
     do {
         if (g.count < NVDR_GN_STARTS) { g.start[g.count] = at; g.left[g.count] = left; }
@@ -582,7 +585,8 @@ template <int P>
 static int gn_norm(const GradList &l, double *part, const GradOut &out, hipStream_t st)
 {
     GradLaunches g;
-    return gn_parts<P>(l, gn_bytes(l), part, true, out, g, st);
+    GradTable tab;
+    return gn_parts<P>(l, gn_bytes(l), part, true, out, g, tab, st);
 }
 
 static int gn_norm_typed(const GradList &l, int norm_type, double *part, const GradOut &out, hipStream_t st)
@@ -607,9 +611,14 @@ static int gn_clip(const GradList &l, double max_norm, double *part, float *norm
     GradLaunches g;
     GradOut out = {};
     out.max_norm = max_norm; out.norm = norm; out.factor = factor;
-    if (int r = gn_parts<P>(l, bytes, part, finish, out, g, st)) return r;
+    if (int r = gn_parts<P>(l, bytes, part, finish, out, g, tab, st)) return r;
     const int n_part = finish ? 0 : g.n_part;
     const bool stream = bytes > NVDR_GN_KEEP;
+    if (g.count == 1 && !stream) {                                  // the table of the norm's one launch is the scaling's
+        if (bytes) grad_scale_kernel<P, false><<<(unsigned)g.n_part, NVDR_GN_BLOCK, 0, st>>>(tab, part, n_part, max_norm, norm, factor);
+        NVDR_LAUNCH_CHECK();
+        return 0;
+    }
     auto launch = [&](int64_t at, int64_t left, int64_t *behind, int64_t *after) -> bool {
         const unsigned blocks = gn_fill(l, &at, &left, stream ? NVDR_GN_STREAM_GRID : NVDR_GN_GRID, tab);
         if (blocks && stream) grad_scale_kernel<P, true><<<blocks, NVDR_GN_STREAM_BLOCK, 0, st>>>(tab, part, n_part, max_norm, norm, factor);

@@ -27,14 +27,17 @@ struct Lists {
     std::vector<int64_t> n;
     std::vector<uint8_t> type;
     std::vector<Py_ssize_t> irregular;              // tensors whose elements do not fill their memory exactly once
-    std::vector<at::Tensor> held;                   // what a call writes to: another thread may drop a parameter's gradient during the call
+    // of a call that writes to them:
+    std::vector<c10::TensorImpl *> written;         // (until Python code or another thread can run)
+    std::vector<c10::Storage> held;                 // their memory: another thread may drop a parameter's gradient during the call
+    bool ordered = true;                            // each begins behind the one before
     int device = -1;
     int64_t count() const { return (int64_t)n.size(); }
 };
 
-// The gradients in `seq`, a list: tensors, or parameters whose gradients are meant (None is left out).  hold: with a reference to each.
-// false: an exception is set.
-bool collect(PyObject *seq, bool grads, bool hold, Lists &l)
+// The gradients in `seq`, a list: tensors, or parameters whose gradients are meant (None is left out).  writes: what the call needs that writes to
+// them (references to the memory, not to each tensor: an atomic a tensor would cost a list of 400 views 3 us).  false: an exception is set.
+bool collect(PyObject *seq, bool grads, bool writes, Lists &l)
 {
     if (!PyList_Check(seq)) {
         PyErr_SetString(PyExc_TypeError, "a list is expected");
@@ -42,13 +45,16 @@ bool collect(PyObject *seq, bool grads, bool hold, Lists &l)
     }
     const size_t most = (size_t)PyList_GET_SIZE(seq);
     l.data.reserve(most); l.n.reserve(most); l.type.reserve(most);
-    if (hold) l.held.reserve(most);
-    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
-        PyObject *item = PyList_GET_ITEM(seq, k);
-        if (!THPVariable_Check(item)) {
-            PyErr_Format(PyExc_TypeError, "gradients must be tensors (got %s)", Py_TYPE(item)->tp_name);
+    if (writes) l.written.reserve(most);
+    const c10::StorageImpl *memory = nullptr;
+    uintptr_t behind = 0;
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k)               // (the check of a subclass runs Python code: in front of everything else)
+        if (!THPVariable_Check(PyList_GET_ITEM(seq, k))) {
+            PyErr_Format(PyExc_TypeError, "gradients must be tensors (got %s)", Py_TYPE(PyList_GET_ITEM(seq, k))->tp_name);
             return false;
         }
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
+        PyObject *item = PyList_GET_ITEM(seq, k);
         const at::Tensor &own = THPVariable_Unpack(item);          // (the list is the caller's own: nobody takes the item out)
         const at::Tensor &t = grads ? own.grad() : own;
         if (!t.defined()) continue;
@@ -65,7 +71,8 @@ bool collect(PyObject *seq, bool grads, bool hold, Lists &l)
             Py_XDECREF(d);
             return false;
         }
-        if (!t.is_cuda() || (l.device >= 0 && t.get_device() != l.device)) {
+        const c10::Device device = t.device();
+        if (!device.is_cuda() || (l.device >= 0 && device.index() != l.device)) {
             PyErr_SetString(PyExc_RuntimeError, "gradients must reside on one GPU; this path has no CPU fallback");
             return false;
         }
@@ -73,12 +80,21 @@ bool collect(PyObject *seq, bool grads, bool hold, Lists &l)
             PyErr_SetString(PyExc_ValueError, "gradients must be dense");
             return false;
         }
-        l.device = (int)t.get_device();
+        l.device = device.index();
         if (!t.is_non_overlapping_and_dense()) l.irregular.push_back((Py_ssize_t)l.n.size());
         l.data.push_back(t.data_ptr());
         l.n.push_back(t.numel());
         l.type.push_back((uint8_t)type);
-        if (hold) l.held.push_back(t);
+        if (writes && t.numel()) {
+            c10::TensorImpl *const impl = t.unsafeGetTensorImpl();
+            l.written.push_back(impl);
+            const c10::Storage &storage = impl->unsafe_storage();
+            if (storage.unsafeGetStorageImpl() != memory) l.held.push_back(storage);
+            memory = storage.unsafeGetStorageImpl();
+            const uintptr_t at = (uintptr_t)l.data.back();
+            l.ordered &= at >= behind;
+            behind = at + (uintptr_t)t.numel() * (type == NVDR_GRAD_F32 ? 4 : 2);
+        }
     }
     return true;
 }
@@ -274,13 +290,23 @@ static PyObject *clip(PyObject *, PyObject *args)
     return guarded([&]() -> PyObject * {
         Lists l;
         if (!collect(seq, grads != 0, true, l)) return nullptr;
-        if (!l.irregular.empty()) {
+        if (!l.irregular.empty() || !l.ordered) {
             size_t i, j;
-            if (!shared(l.held, &i, &j)) return irregular_list(l);
-            return i == j ? PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
+            std::vector<at::Tensor> tensors;
+            for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
+                const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(seq, k));
+                if (!grads || t.grad().defined()) tensors.push_back(grads ? t.grad() : t);
+            }
+            if (!shared(tensors, &i, &j)) {
+                if (!l.irregular.empty()) return irregular_list(l);
+            } else return i == j ? PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
                           : PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: two gradients share memory (the same tensor twice, or overlapping views)");
         }
         if (l.device < 0) Py_RETURN_NONE;
+        // versions go up, as with any operation in place: the call is accepted (the library's checks are of the lists above)
+        for (c10::TensorImpl *t : l.written)
+            if (!t->is_inference()) t->bump_version();
+        l.written.clear();
         const c10::DeviceGuard device(at::Device(at::kCUDA, (at::DeviceIndex)l.device));
         void *stream;
         if (!current_stream(l.device, &stream)) return nullptr;
@@ -295,9 +321,6 @@ static PyObject *clip(PyObject *, PyObject *args)
         rc = grad_clip_entry(l.data.data(), l.n.data(), l.type.data(), l.count(), code, max_norm, w, size, at, stream);
         Py_END_ALLOW_THREADS
         if (rc) return failed("clip_grad_norm_", rc);
-        // versions go up, as with any operation in place -- not before the call has been accepted
-        for (const at::Tensor &t : l.held)
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
         return THPVariable_Wrap(result);
     });
 }

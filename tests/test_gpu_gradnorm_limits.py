@@ -287,3 +287,18 @@ def test_bounds_on_the_host_are_refused(dev):
         with pytest.raises(ValueError, match='bounds of parameter 0'):
             _adam([torch.zeros(5, 3)], dev, clamps=[c])
     _adam([torch.zeros(5, 3)], dev, clamps=[(None, None, bound.to(dev))])
+
+
+def test_parameters_of_a_subclass(dev):
+    """Asking whether a subclass is a tensor may run Python code."""
+    from nvdiffrecmc_amd.optim import clip_grad_norm_, grad_norm
+
+    class Mine(torch.Tensor):
+        pass
+    p = torch.nn.Parameter(torch.zeros(5, device=dev))
+    q = torch.zeros(3, device=dev).as_subclass(Mine).requires_grad_(True)
+    p.grad, q.grad = torch.full((5,), 2.0, device=dev), torch.full((3,), 2.0, device=dev)
+    assert float(grad_norm([p.grad, q.grad])) == float(clip_grad_norm_([p, q], 1.0)) == torch.tensor(32.0).sqrt().item()
+    assert abs(float(q.grad[0]) - 2.0 / math.sqrt(32.0)) < 1e-6
+    with pytest.raises(TypeError, match='int'):
+        clip_grad_norm_([p, q, 1], 1.0)

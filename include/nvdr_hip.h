@@ -471,9 +471,10 @@ typedef struct nvdr_adam_tensor {
                                (Texture2D.normalize_ of the normal map, train.py:473-474) */
     uint8_t *active;        /* optional (n % 3 == 0): one byte per tile of 64 three-channel texels, zero-initialised by the caller once.  Tiles
                                whose gradient is all zero and that never had a non-zero one are skipped after step 1 (their update is the
-                               identity): the sparse gradients of a nearest-texel texture lookup.  NULL: every element is updated */
+                               identity; a step whose grad_scale * factor is not finite visits every tile): the sparse gradients of a
+                               nearest-texel texture lookup.  NULL: every element is updated */
     int32_t zero_grad;      /* with `active`: the gradient of every updated tile is zeroed behind the update (`grad` is written) */
-    int32_t frozen;         /* != 0: the tensor is left alone altogether (parameter, moments and gradient untouched) */
+    int32_t frozen;         /* != 0: parameter and moments are left alone, and the gradient too unless zero_grad clears it */
 } nvdr_adam_tensor;
 /* sizeof of the argument blocks as THIS build of the library sees them: a caller compiled (or a ctypes mirror written) against another
  * revision of this header compares before its first call.  which: 0 nvdr_adam_tensor, 1 nvdr_env_shade_args, 2 nvdr_texture_args,
@@ -487,7 +488,7 @@ int nvdr_adam_step(const nvdr_adam_tensor *tensors, int n_tensors, double lr, do
 int nvdr_adam_step_partial(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps, int *state,
                            int advance, void *stream);
 
-/* The same update with every gradient also multiplied by *grad_factor (device memory, read by the launch; NULL: one): the factor of
+/* The same update with every gradient multiplied by grad_scale * *grad_factor, one product (device memory, read by the launch; NULL: one): the factor of
  * nvdr_grad_norm, so that clipping takes no pass of its own over the gradients.  The gradients themselves stay as they are. */
 int nvdr_adam_step_factor(const nvdr_adam_tensor *tensors, int n_tensors, double lr, double beta1, double beta2, double eps, int *state,
                           int advance, const float *grad_factor, void *stream);
@@ -501,8 +502,8 @@ int nvdr_adam_step_clipped(const nvdr_adam_tensor *tensors, int n_tensors, doubl
  *     norm   = (sum_k sum_i |scale[k] data[k][i]|^p)^(1/p), p = 1 or 2; the largest magnitude for NVDR_NORM_INF (a NaN anywhere gives a NaN)
  *     factor = min(1, max_norm / (norm + 1e-6)); one for an infinite max_norm
  * data[k]: n[k] contiguous elements of type[k] in any mixture, aligned to their own size; n[k] = 0 is skipped.  scale: NULL for ones.  The
- * four lists live in HOST memory and are read before the call returns (a captured graph keeps them).  Sums in fp64, in an order that depends
- * on sizes and alignment only.  workspace: nvdr_grad_norm_workspace(n, type, n_tensors, clip) doubles of device memory (none for a short list
+ * four lists live in HOST memory and are read before the call returns (a captured graph keeps them).  Sums in fp64, in an order that
+ * depends on sizes, alignment and which tensors are neighbours in memory.  workspace: nvdr_grad_norm_workspace(n, type, n_tensors, clip) doubles of device memory (none for a short list
  * that is clipped, which one workgroup does), 8-byte aligned, nothing to initialise; launches that may run at the same time need one each.  norm, factor: one float each in device memory (factor may be NULL).
  * nvdr_grad_norm leaves the gradients alone; nvdr_grad_clip multiplies them by the factor in place (computed in fp32, one rounding to the
  * element's type) and writes nothing when the factor is one.  Gradients of nvdr_grad_clip must not share memory. */

@@ -9,8 +9,9 @@
 //
 // Sums in fp64.  An fp32 gradient's square leaves the range of fp32 from 1.8e19 up and 1e-19 down, and a sum of 1e9 terms loses half of
 // fp32's digits; a conversion and an fma in fp64 per element are far below what the memory can deliver in elements.  No atomics: every
-// workgroup writes its sum to a place of its own and they are added in a fixed order, so that a result depends on the values, the sizes
-// and the alignment alone.
+// workgroup writes its sum to a place of its own and they are added in a fixed order.  The order follows from the sizes, the alignment, which
+// tensors are neighbours in memory (they are cut as one) and whether one workgroup clips the list: the same call on the same places gives
+// the same bits, and other places change a norm by the rounding of its fp64 sum, which is seen in fp32 once in some 1e8 times.
 //
 // Work split.  The tensors are cut into chunks of NVDR_GN_CHUNK bytes, and runs of chunks, whatever tensors they fall into, are dealt to the
 // workgroups in turn, as many rounds of equally long runs as NVDR_GN_RUN gives: a long tensor is shared by many workgroups, many short ones

@@ -10,8 +10,8 @@
 //     m = m + (g - m) * (1 - b1);  v = v * b2 + (1 - b2) * g * g
 //     p = p - (lr / (1 - b1^t)) * m / (sqrt(v) / sqrt(1 - b2^t) + eps);  p = max(min(p, hi), lo)
 //
-// With clipping (nvdr_adam_step_clipped) the norm of the effective gradients comes first (gradnorm.hip) and its factor enters g: the gradients
-// are read once more, not written, and no launch follows for the step counter.
+// With clipping (nvdr_adam_step_clipped) the norm of the effective gradients comes first (gradnorm.hip) and its factor enters g, as one product
+// with the scale (an outlier times the scale alone can leave fp32 where its clipped value does not): the gradients are read once more, not written, and no launch follows for the step counter.
 //
 // Bytes bound it: 28 per parameter.  10.7 M parameters of the scene's set, 298 MB: 72 us with one element a lane and access, 64 us with
 // sixteen bytes, 48 us (6.2 TB/s, what a large copy reaches) with the moments past the caches.  Textures by tiles (12 bytes a texel where
@@ -133,7 +133,7 @@ __device__ __forceinline__ void adam_texel(const nvdr_adam_tensor &T, const Adam
     adam_store<false>(p, T.param + e);
 }
 
-// begin: what grad_norm_final_kernel has prepared of this step (the counter has moved already); NULL: from state, with *grad_factor
+// begin: what the kernel that finished the norm has prepared of this step (the counter has moved already); NULL: from state, with *grad_factor
 template <bool STREAM>
 __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, double lr, double beta1d, double beta2d, float eps, const int *state,
                                                                 const float *grad_factor, const AdamStep *begin)
@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(ADAM_BLOCK) adam_step_kernel(AdamTable tab, do
 }
 
 // The step counter and the running powers move in a launch of their own (one thread, ~4 us) behind the update: every workgroup of the
-// update has read them by then (stream order).  Rounds 2-3 let the workgroups of the update draw tickets on ONE word and the last
-// one publish the state: up to 2 048 same-address atomics, which retire one every ~12 ns -- 25 us of a 33 us kernel.  (A clipped step of all
+// update has read them by then (stream order).  Tickets that the workgroups of the update draw on ONE word, the last one
+// publishing the state, cost more: up to 2 048 same-address atomics, which retire one every ~12 ns -- 25 us of a 33 us kernel.  (A clipped step of all
 // tensors needs no launch for it: the kernel that finishes the norm prepares the step and moves the counter.)
 __global__ void adam_advance_kernel(int *state, double beta1d, double beta2d) { adam_advance(state, beta1d, beta2d); }
 

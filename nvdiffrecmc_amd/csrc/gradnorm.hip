@@ -481,7 +481,7 @@ static int gn_check_apart(const GradList &l, const char *who)
     int64_t m = 0;
     for (int64_t k = 0; k < l.count; ++k)
         if (l.n[k]) s[m++] = Span((uintptr_t)l.data[k], (uintptr_t)l.data[k] + (uintptr_t)(l.n[k] * gn_size(l.type[k])));
-    std::sort(s, s + m);
+    std::sort(s, s + m, [](const Span &a, const Span &b) { return a.first < b.first; });      // (none is empty: equal beginnings overlap)
     bool apart = true;
     for (int64_t k = 1; k < m; ++k) apart = apart && s[k].first >= s[k - 1].second;
     free(s);

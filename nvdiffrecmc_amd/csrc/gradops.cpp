@@ -30,7 +30,6 @@ struct Lists {
     // of a call that writes to them:
     std::vector<c10::TensorImpl *> written;         // (until Python code or another thread can run)
     std::vector<c10::Storage> held;                 // their memory: another thread may drop a parameter's gradient during the call
-    bool ordered = true;                            // each begins behind the one before
     int device = -1;
     int64_t count() const { return (int64_t)n.size(); }
 };
@@ -47,7 +46,6 @@ bool collect(PyObject *seq, bool grads, bool writes, Lists &l)
     l.data.reserve(most); l.n.reserve(most); l.type.reserve(most);
     if (writes) l.written.reserve(most);
     const c10::StorageImpl *memory = nullptr;
-    uintptr_t behind = 0;
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k)               // (the check of a subclass runs Python code: in front of everything else)
         if (!THPVariable_Check(PyList_GET_ITEM(seq, k))) {
             PyErr_Format(PyExc_TypeError, "gradients must be tensors (got %s)", Py_TYPE(PyList_GET_ITEM(seq, k))->tp_name);
@@ -91,9 +89,6 @@ bool collect(PyObject *seq, bool grads, bool writes, Lists &l)
             const c10::Storage &storage = impl->unsafe_storage();
             if (storage.unsafeGetStorageImpl() != memory) l.held.push_back(storage);
             memory = storage.unsafeGetStorageImpl();
-            const uintptr_t at = (uintptr_t)l.data.back();
-            l.ordered &= at >= behind;
-            behind = at + (uintptr_t)t.numel() * (type == NVDR_GRAD_F32 ? 4 : 2);
         }
     }
     return true;
@@ -290,23 +285,23 @@ static PyObject *clip(PyObject *, PyObject *args)
     return guarded([&]() -> PyObject * {
         Lists l;
         if (!collect(seq, grads != 0, true, l)) return nullptr;
-        if (!l.irregular.empty() || !l.ordered) {
-            size_t i, j;
+        auto gradient = [&](Py_ssize_t k) -> const at::Tensor & {
+            const at::Tensor &own = THPVariable_Unpack(PyList_GET_ITEM(seq, k));
+            return grads ? own.grad() : own;
+        };
+        if (!l.irregular.empty()) {
             std::vector<at::Tensor> tensors;
-            for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
-                const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(seq, k));
-                if (!grads || t.grad().defined()) tensors.push_back(grads ? t.grad() : t);
-            }
-            if (!shared(tensors, &i, &j)) {
-                if (!l.irregular.empty()) return irregular_list(l);
-            } else return i == j ? PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
+            for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k)
+                if (gradient(k).defined()) tensors.push_back(gradient(k));
+            size_t i, j;
+            if (!shared(tensors, &i, &j)) return irregular_list(l);
+            return i == j ? PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: a gradient whose elements share memory (an expanded tensor) cannot be scaled in place")
                           : PyErr_Format(PyExc_RuntimeError, "clip_grad_norm_: two gradients share memory (the same tensor twice, or overlapping views)");
         }
         if (l.device < 0) Py_RETURN_NONE;
-        // versions go up, as with any operation in place: the call is accepted (the library's checks are of the lists above)
+        // versions go up, as with any operation in place
         for (c10::TensorImpl *t : l.written)
             if (!t->is_inference()) t->bump_version();
-        l.written.clear();
         const c10::DeviceGuard device(at::Device(at::kCUDA, (at::DeviceIndex)l.device));
         void *stream;
         if (!current_stream(l.device, &stream)) return nullptr;
@@ -320,6 +315,16 @@ static PyObject *clip(PyObject *, PyObject *args)
         Py_BEGIN_ALLOW_THREADS
         rc = grad_clip_entry(l.data.data(), l.n.data(), l.type.data(), l.count(), code, max_norm, w, size, at, stream);
         Py_END_ALLOW_THREADS
+        if (rc == -1) {                     // refused, nothing written: they come down again (of gradients that are still the parameters')
+            size_t at = 0;
+            for (Py_ssize_t k = 0; k < PyList_GET_SIZE(seq); ++k) {
+                const at::Tensor &t = gradient(k);
+                if (at >= l.written.size() || t.unsafeGetTensorImpl() != l.written[at]) continue;
+                ++at;
+                c10::VariableVersion version = t.unsafeGetTensorImpl()->version_counter();
+                if (!t.is_inference() && version.current_version() > 0) version.set_version((int64_t)version.current_version() - 1);
+            }
+        }
         if (rc) return failed("clip_grad_norm_", rc);
         return THPVariable_Wrap(result);
     });

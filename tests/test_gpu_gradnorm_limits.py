@@ -302,3 +302,34 @@ def test_parameters_of_a_subclass(dev):
     assert abs(float(q.grad[0]) - 2.0 / math.sqrt(32.0)) < 1e-6
     with pytest.raises(TypeError, match='int'):
         clip_grad_norm_([p, q, 1], 1.0)
+
+
+@pytest.mark.parametrize('order', ['as they lie', 'backwards', 'shuffled'])
+def test_the_order_of_a_list_does_not_matter(order, dev):
+    """Neighbours, gaps and tensors of their own, in any order: scaled once, versions raised once, and refused with one of them twice."""
+    from nvdiffrecmc_amd.optim import clip_grad_norm_
+    buf = torch.zeros(40000, device=dev)
+    sizes = [1, 700, 0, 3000, 5, 64, 9000]
+    at, grads = 3, []
+    for k, n in enumerate(sizes):
+        grads.append(buf[at:at + n])
+        at += n + (k % 2) * 7
+    grads += [torch.zeros(n, device=dev) for n in (11, 30000, 2)]
+    if order != 'as they lie':
+        grads.sort(key=lambda g: -g.data_ptr())
+    if order == 'shuffled':
+        grads = grads[1::2] + grads[::2]
+    host = [_values(g.shape, 3 + k) for k, g in enumerate(grads)]
+    for g, h in zip(grads, host):
+        g.copy_(h)
+    norm = math.sqrt(sum(float((h.double() ** 2).sum()) for h in host))
+    with pytest.raises(RuntimeError, match='share memory'):
+        clip_grad_norm_(_with_grads(grads + [grads[-1] if grads[-1].numel() else grads[0]]), 0.5 * norm)
+    ps, versions = _with_grads(grads), {id(g): g._version for g in grads if g.untyped_storage().data_ptr() != buf.untyped_storage().data_ptr()}
+    got = clip_grad_norm_(ps, 0.5 * norm)
+    assert abs(got.item() - norm) <= (2.0 ** -24 + 1e-10) * norm
+    factor = 0.5 * norm / (norm + 1e-6)
+    for g, h in zip(grads, host):
+        x = h.double() * factor
+        assert bool(((g.cpu().double() - x).abs() <= 2.0 ** -23 * x.abs() + 2.0 ** -150).all())
+        assert g._version == versions.get(id(g), g._version - 1) + 1

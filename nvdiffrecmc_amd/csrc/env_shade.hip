@@ -203,6 +203,12 @@ __global__ void __launch_bounds__(256) zero_outputs_kernel(float *b0, float *b1,
     }
 }
 
+// every tag of the light gradient's record blocks: "no records"
+__global__ void __launch_bounds__(256) no_records_kernel(uint16_t *tags, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) tags[i] = 0xFFFFu;
+}
+
 __global__ void begin_launch_kernel(unsigned *pix_count, unsigned *chunk_counts, int n_chunks, int reuse, unsigned cap, unsigned seg_cap,
                                     unsigned *seed_counter, unsigned *seed_snapshot, unsigned seed_advance)
 {
@@ -2329,7 +2335,8 @@ static int env_shade_launch(nvdr_ctx *c, const nvdr_env_shade_args *a, bool back
     p.lg_spare_base = (unsigned)(own_slots >> 7);
     p.lg_spw = lg_spw;
     if (backward && lg_records) {
-        if (c->lg_tags_dirty) NVDR_HIP_TRY(hipMemsetAsync(c->lg_tags, 0xFF, sizeof(uint16_t) * c->lg_tags_cap, stream));
+        // (a kernel: the first backward pass behind a forward pass that made the array may be captured)
+        if (c->lg_tags_dirty) no_records_kernel<<<min(div_up((int64_t)c->lg_tags_cap, 1024), 1024u), 256, 0, stream>>>(c->lg_tags, (int64_t)c->lg_tags_cap);
         c->lg_tags_dirty = true;        // until the gather of the last chunk has been enqueued
     }
     p.pix_list = c->pix_list;

@@ -37,3 +37,15 @@ def test_tools_that_are_named_exist():
 def test_no_build_switch_leaves_work_out():
     """A build that skips work to time the rest has no place in the sources."""
     assert not [f for f in _files('.hip', '.h', '.cpp') if re.search(r'#define \w*(SKIP|EXPERIMENT)\w*', open(f).read())]
+
+
+def test_no_memset_node_on_a_path_that_may_be_captured():
+    """A memset inside a captured graph has given wrong results on replays: the library fills by kernels, but for the experiment switches and the
+    arithmetic's self-test, which is not captured."""
+    found = []
+    for f in _files('.hip', '.h'):
+        if 'ubench' in f:
+            continue
+        lines = open(f).read().splitlines()
+        found += [(os.path.basename(f), line.strip()) for k, line in enumerate(lines) if 'hipMemsetAsync(' in line and 'c->debug &' not in line + lines[max(k - 1, 0)]]
+    assert [(f, 'counters' in line) for f, line in found] == [('core.hip', True)], found
